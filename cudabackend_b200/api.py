@@ -15,8 +15,8 @@ STATUS_NAMES = ["SUCCESS", "ALLOC_FAILED", "BAD_ALLOC", "FREE_FAILED", "BAD_PARA
                 "UNSUPPORTED_DATATYPE", "EXECUTION_FAILED", "INSUFFICIENT_DRIVER", "DEVICE_TYPE_MISMATCH"]
 STATUS = {name: i for i, name in enumerate(STATUS_NAMES)}
 DTYPES = {"unknown": 0, "uint8": 1, "int8": 2, "int16": 3, "int32": 4, "int64": 5, "float16": 6, "bfloat16": 7, "float32": 8, "float64": 9,
-          "complex32": 10, "complex64": 11}
-DTYPE_SIZES = {"uint8": 1, "int8": 1, "int16": 2, "int32": 4, "int64": 8, "float16": 2, "bfloat16": 2, "float32": 4, "float64": 8}
+          "complex32": 10, "complex64": 11, "float8_e4m3": 12}
+DTYPE_SIZES = {"float8_e4m3": 1, "uint8": 1, "int8": 1, "int16": 2, "int32": 4, "int64": 8, "float16": 2, "bfloat16": 2, "float32": 4, "float64": 8}
 ACTIVATIONS = {"linear": 0, "sigmoid": 1, "tanh": 2, "relu": 3, "selu": 4, "elu": 5, "exponential": 6, "softplus": 7, "softsign": 8}
 CONVOLUTION_MODE, CROSS_CORRELATION_MODE = 0, 1
 GEMM_N, GEMM_T = 0, 1
@@ -90,6 +90,9 @@ SIGNATURES = {
     "cudaOptimizerLearn": (_INT, [_H, _H, _VP, _H, _H, _VP, _H, _H, _H]),
     "cudaAddBias": (_INT, [_H, _VP, _VP, _H, _H, _H, _H, _H, _H, _VP, _VP, _VP, _H, _INT]),
     "cudaActivationForward": (_INT, [_H, _INT, _VP, _H, _H, _VP, _H, _H]),
+    "cudaQuantizeBlocks": (_INT, [_H, _H, _H, _H, _H, _H, _H]),
+    "cudaRmsNormQuantize": (_INT, [_H, _H, _H, _H, _H, _H, _H, ctypes.c_double, _H, _H, _H, _H]),
+    "cudaGemmBlockScaled": (_INT, [_H, _INT, _INT, _VP, _H, _H, _H, _H, _H, _H, _H, _H, _VP, _H, _H]),
 }
 
 # exported for link compatibility, return NOT_SUPPORTED
@@ -364,6 +367,35 @@ def bfloat16_bits_to_float(b):
     return (np.ascontiguousarray(b, dtype=np.uint16).astype(np.uint32) << 16).view(np.float32)
 
 
+def _float8_values():
+    """The value of every e4m3 code (float64); code 0x7F / 0xFF is NaN."""
+    code = np.arange(256)
+    exponent, mantissa = (code >> 3) & 15, (code & 7).astype(np.float64)
+    magnitude = np.where(exponent == 0, np.ldexp(mantissa, -9), np.ldexp(8.0 + mantissa, exponent - 10))
+    magnitude[(code & 0x7F) == 0x7F] = np.nan
+    return np.where(code & 0x80, -magnitude, magnitude)
+
+
+FLOAT8_VALUES = _float8_values()
+
+
+def float_to_float8_bits(a):
+    """float -> e4m3 codes (uint8): round to nearest, ties to even, magnitudes past 448 saturate, NaN stays NaN."""
+    a = np.asarray(a, dtype=np.float64)
+    grid = FLOAT8_VALUES[:0x7F]
+    m = np.minimum(np.abs(np.where(np.isnan(a), 0.0, a)), grid[-1])
+    low = np.searchsorted(grid, m, side="right") - 1
+    high = np.minimum(low + 1, 0x7E)
+    below, above = m - grid[low], grid[high] - m
+    code = np.where((above < below) | ((above == below) & (low & 1 == 1)), high, low)
+    code = np.where(np.isnan(a), 0x7F, code)
+    return (code | np.where(np.signbit(a), 0x80, 0)).astype(np.uint8)
+
+
+def float8_bits_to_float(b):
+    return FLOAT8_VALUES[np.ascontiguousarray(b, dtype=np.uint8)]
+
+
 def to_storage(a, dtype):
     """Rounds a float array to the storage dtype; returns (array to upload, the same values as float64)."""
     if dtype == "float16":
@@ -372,6 +404,9 @@ def to_storage(a, dtype):
     if dtype == "bfloat16":
         s = float_to_bfloat16_bits(a)
         return s, bfloat16_bits_to_float(s).astype(np.float64)
+    if dtype == "float8_e4m3":
+        s = float_to_float8_bits(a)
+        return s, float8_bits_to_float(s)
     if dtype == "float32":
         s = np.ascontiguousarray(a, dtype=np.float32)
         return s, s.astype(np.float64)
@@ -386,13 +421,15 @@ def to_storage(a, dtype):
 
 def host_buffer(shape, dtype):
     np_dtype = {"float16": np.float16, "bfloat16": np.uint16, "float32": np.float32, "float64": np.float64, "int8": np.int8,
-                "int32": np.int32}[dtype]
+                "int32": np.int32, "float8_e4m3": np.uint8}[dtype]
     return np.empty(shape, dtype=np_dtype)
 
 
 def from_storage(a, dtype):
     if dtype == "bfloat16":
         return bfloat16_bits_to_float(a).astype(np.float64)
+    if dtype == "float8_e4m3":
+        return float8_bits_to_float(a)
     return np.asarray(a).astype(np.float64)
 
 

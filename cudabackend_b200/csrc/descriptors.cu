@@ -27,6 +27,7 @@ namespace avocado
 				{
 					case AVOCADO_DTYPE_UINT8:
 					case AVOCADO_DTYPE_INT8:
+					case AVOCADO_DTYPE_FLOAT8_E4M3:
 						return 1;
 					case AVOCADO_DTYPE_INT16:
 					case AVOCADO_DTYPE_FLOAT16:

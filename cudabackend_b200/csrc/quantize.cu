@@ -1,0 +1,529 @@
+/*
+ * quantize.cu -- cudaQuantizeBlocks and cudaRmsNormQuantize: what turns 16-bit or float32 tensors into the e4m3 codes and
+ * float32 block scales that cudaGemmBlockScaled reads.  No counterpart in the reference.
+ *
+ *   block of 128 elements:  amax = max |x|,  a = max(amax, 2^-100),  scale = a / 448,  code = e4m3_rne(x * (448 / a))
+ *   norm:                   h = x + z,  y = h * (1 / sqrt(mean(h^2) + eps)) * gamma,  then the same on y
+ *
+ * Both move every element once: the inputs are read into registers, reduced, scaled and written from there.  A block of 128
+ * elements belongs to 16 neighbouring lanes (half a warp) with eight elements each: 16 bytes of a 16-bit tensor per load, 8
+ * bytes of codes per store, and the maximum over the block is four shuffles.  Magnitudes are compared as integers (the bit
+ * pattern without its sign grows with the magnitude and puts NaN above infinity), so one NaN reaches its block's scale.
+ * One division per block; the product x * (448 / a) is at most 448 * (1 + 2^-23), which rounds to 448, so nothing saturates.
+ */
+#include <Avocado/cuda_backend_ext.h>
+
+#include "block_scaled.hpp"
+#include "device_utils.cuh"
+#include "objects.hpp"
+
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <cmath>
+
+namespace
+{
+	using namespace avocado::backend;
+	using namespace avocado::backend::b200;
+	using namespace bk;
+
+	constexpr int kLanes = 16;   /* lanes that share one block of 128 elements */
+	constexpr int kPerLane = 8;  /* elements of it per lane */
+	constexpr int kThreads = 256;
+	constexpr int kMaxQuantizedRow = 1 << 30; /* column indices, rounded up to whole blocks, stay in 32 bits */
+	constexpr int kMaxNormedRow = 1 << 20;    /* a thread adds up at most 1024 squares: the sum keeps about 20 of its 24 bits */
+	constexpr unsigned kFullWarp = 0xFFFFFFFFu;
+
+	__device__ __forceinline__ uint32_t magnitude_bits(float x)
+	{
+		return __float_as_uint(x) & 0x7FFFFFFFu;
+	}
+	__device__ __forceinline__ uint32_t max_over_half_warp(uint32_t v)
+	{
+#pragma unroll
+		for (int i = kLanes / 2; i > 0; i /= 2)
+			v = max(v, __shfl_xor_sync(kFullWarp, v, i));
+		return v;
+	}
+	/* the clamped maximum as a float; NaN passes (its bit pattern is above that of 2^-100) */
+	__device__ __forceinline__ float clamped_amax(uint32_t bits)
+	{
+		return __uint_as_float(max(bits, __float_as_uint(kSmallestAmax)));
+	}
+	__device__ __forceinline__ uint32_t four_codes(const float *x, float r)
+	{
+		const uint32_t low = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[0], r), __fmul_rn(x[1], r)), __NV_SATFINITE, __NV_E4M3);
+		const uint32_t high = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[2], r), __fmul_rn(x[3], r)), __NV_SATFINITE, __NV_E4M3);
+		return low | (high << 16);
+	}
+
+	/* The eight elements of lane `l` of the block that starts at column `first`: consecutive ones where rows can be moved in
+	 * 16-byte pieces (VEC), every 16th otherwise, so that neighbouring lanes touch neighbouring elements either way. */
+	template<bool VEC>
+	__device__ __forceinline__ int column_of(int first, int l, int i)
+	{
+		return VEC ? first + l * kPerLane + i : first + l + i * kLanes;
+	}
+	template<bool VEC, typename T>
+	__device__ __forceinline__ void load_eight(float (&v)[kPerLane], const T *row, int first, int l, int columns)
+	{
+		if constexpr (VEC)
+		{
+			const int column = first + l * kPerLane;
+			if (column < columns) /* VEC: columns is a multiple of eight */
+			{
+				constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
+#pragma unroll
+				for (int j = 0; j < kPerLane; j += kPiece)
+				{
+					const Vec<T, kPiece> piece = load_vec<T, kPiece>(row + column + j);
+#pragma unroll
+					for (int i = 0; i < kPiece; i++)
+						v[j + i] = to_compute(piece.v[i]);
+				}
+			}
+			else
+			{
+#pragma unroll
+				for (int i = 0; i < kPerLane; i++)
+					v[i] = 0.0f;
+			}
+		}
+		else
+		{
+#pragma unroll
+			for (int i = 0; i < kPerLane; i++)
+			{
+				const int column = column_of<VEC>(first, l, i);
+				v[i] = column < columns ? to_compute(row[column]) : 0.0f;
+			}
+		}
+	}
+	template<bool VEC, typename T>
+	__device__ __forceinline__ void store_eight(T *row, const float (&v)[kPerLane], int first, int l, int columns)
+	{
+		if constexpr (VEC)
+		{
+			const int column = first + l * kPerLane;
+			if (column < columns)
+			{
+				constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
+#pragma unroll
+				for (int j = 0; j < kPerLane; j += kPiece)
+				{
+					Vec<T, kPiece> piece;
+#pragma unroll
+					for (int i = 0; i < kPiece; i++)
+						piece.v[i] = from_compute<T>(v[j + i]);
+					store_vec<T, kPiece>(row + column + j, piece);
+				}
+			}
+		}
+		else
+		{
+#pragma unroll
+			for (int i = 0; i < kPerLane; i++)
+			{
+				const int column = column_of<VEC>(first, l, i);
+				if (column < columns)
+					row[column] = from_compute<T>(v[i]);
+			}
+		}
+	}
+	template<bool VEC>
+	__device__ __forceinline__ void store_codes(uint8_t *row, const float (&v)[kPerLane], float r, int first, int l, int columns)
+	{
+		const uint2 codes = make_uint2(four_codes(v, r), four_codes(v + 4, r));
+		if constexpr (VEC)
+		{
+			const int column = first + l * kPerLane;
+			if (column < columns)
+				*reinterpret_cast<uint2*>(row + column) = codes;
+		}
+		else
+		{
+#pragma unroll
+			for (int i = 0; i < kPerLane; i++)
+			{
+				const int column = column_of<VEC>(first, l, i);
+				if (column < columns)
+					row[column] = static_cast<uint8_t>((i < 4 ? codes.x : codes.y) >> (8 * (i % 4)));
+			}
+		}
+	}
+	__device__ __forceinline__ float largest_magnitude(const float (&v)[kPerLane], uint32_t &bits)
+	{
+#pragma unroll
+		for (int i = 0; i < kPerLane; i++)
+			bits = max(bits, magnitude_bits(v[i]));
+		return __uint_as_float(bits);
+	}
+
+	/* ---- 1 x 128 blocks: half a warp per block, no block-wide step ------------------------------------------------ */
+	template<typename T, bool VEC>
+	__global__ void __launch_bounds__(kThreads) kernel_quantize_rows(const T *__restrict__ x, uint8_t *__restrict__ y, float *__restrict__ scales,
+			long long total, int columns, int blocks)
+	{
+		chain_release();
+		chain_wait();
+		const int l = threadIdx.x % kLanes;
+		const long long stride = static_cast<long long>(gridDim.x) * (kThreads / kLanes);
+		for (long long first = static_cast<long long>(blockIdx.x) * (kThreads / kLanes); first < total; first += stride)
+		{
+			const long long b = first + threadIdx.x / kLanes;
+			const bool inside = b < total;
+			const long long row = inside ? b / blocks : 0;
+			const int column = inside ? static_cast<int>(b - row * blocks) * kScaleBlock : columns;
+			float v[kPerLane];
+			load_eight<VEC>(v, x + row * columns, column, l, columns);
+			uint32_t bits = 0;
+			largest_magnitude(v, bits);
+			const float amax = clamped_amax(max_over_half_warp(bits));
+			store_codes<VEC>(y + row * columns, v, kLargestE4m3 / amax, column, l, columns);
+			if (inside and l == 0)
+				scales[b] = amax / kLargestE4m3;
+		}
+	}
+
+	/* ---- 128 x 128 blocks: one thread block each, held in registers between the maximum and the codes ------------------ */
+	template<typename T, bool VEC>
+	__global__ void __launch_bounds__(kThreads) kernel_quantize_squares(const T *__restrict__ x, uint8_t *__restrict__ y, float *__restrict__ scales,
+			long long total, long long rows, int columns, int blocks)
+	{
+		constexpr int kRowsPerPass = kThreads / kLanes;
+		constexpr int kPasses = kScaleBlock / kRowsPerPass;
+		__shared__ uint32_t warp_max[2][kThreads / 32];
+		chain_release();
+		chain_wait();
+		const int l = threadIdx.x % kLanes;
+		int turn = 0;
+		for (long long b = blockIdx.x; b < total; b += gridDim.x, turn ^= 1)
+		{
+			const long long block_row = b / blocks;
+			const int column = static_cast<int>(b - block_row * blocks) * kScaleBlock;
+			const long long row0 = block_row * kScaleBlock + threadIdx.x / kLanes;
+			float v[kPasses][kPerLane];
+			uint32_t bits = 0;
+#pragma unroll
+			for (int p = 0; p < kPasses; p++)
+			{
+				const long long row = row0 + p * kRowsPerPass;
+				load_eight<VEC>(v[p], x + (row < rows ? row : 0) * columns, row < rows ? column : columns, l, columns);
+			}
+#pragma unroll
+			for (int p = 0; p < kPasses; p++)
+				largest_magnitude(v[p], bits);
+			bits = __reduce_max_sync(kFullWarp, bits);
+			if (threadIdx.x % 32 == 0)
+				warp_max[turn][threadIdx.x / 32] = bits;
+			__syncthreads(); /* two sets of slots: the next turn's writes cannot meet this turn's reads */
+#pragma unroll
+			for (int w = 0; w < kThreads / 32; w++)
+				bits = max(bits, warp_max[turn][w]);
+			const float amax = clamped_amax(bits);
+			const float r = kLargestE4m3 / amax;
+#pragma unroll
+			for (int p = 0; p < kPasses; p++)
+			{
+				const long long row = row0 + p * kRowsPerPass;
+				if (row < rows)
+					store_codes<VEC>(y + row * columns, v[p], r, column, l, columns);
+			}
+			if (threadIdx.x == 0)
+				scales[b] = amax / kLargestE4m3;
+		}
+	}
+
+	/* ---- norm + quantise ------------------------------------------------------------------------------------------------
+	 * `warps` warps (a power of two) share a row; half-warp i of them owns the blocks i, i + 2 * warps, ... .  ITEMS > 0: at most
+	 * ITEMS blocks per half-warp, kept in registers between the sum of squares and the codes.  ITEMS = 0: rows of any length,
+	 * read twice. */
+	template<typename T, int ITEMS, bool VEC>
+	__global__ void __launch_bounds__(1024) kernel_rms_norm_quantize(const T *x, const T *z, T *h, const float *__restrict__ gamma, uint8_t *__restrict__ y,
+			float *__restrict__ scales, long long rows, int columns, int blocks, int warps, float epsilon)
+	{
+		__shared__ float warp_sum[32];
+		chain_release();
+		chain_wait();
+		const int warp = threadIdx.x / 32;
+		const int l = threadIdx.x % kLanes;
+		const int warp_in_row = warp & (warps - 1);
+		const int half = warp_in_row * 2 + (threadIdx.x % 32) / kLanes;
+		const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / (32 * warps)) + warp / warps;
+		const bool inside = row < rows;
+		const int limit = inside ? columns : 0; /* a row past the end has no columns: nothing is read or written for it */
+		const long long offset = inside ? row * columns : 0;
+
+		auto load_sum = [&](float (&v)[kPerLane], int column)
+		{
+			load_eight<VEC>(v, x + offset, column, l, limit);
+			if (z != nullptr)
+			{
+				float other[kPerLane];
+				load_eight<VEC>(other, z + offset, column, l, limit);
+#pragma unroll
+				for (int i = 0; i < kPerLane; i++)
+					v[i] += other[i];
+			}
+		};
+		auto finish = [&](float (&v)[kPerLane], int b, float rstd)
+		{
+			const int column = b * kScaleBlock;
+			if (h != nullptr)
+				store_eight<VEC>(h + offset, v, column, l, limit);
+			float g[kPerLane];
+			load_eight<VEC>(g, gamma, column, l, limit);
+			uint32_t bits = 0;
+#pragma unroll
+			for (int i = 0; i < kPerLane; i++)
+				v[i] = __fmul_rn(__fmul_rn(v[i], rstd), g[i]);
+			largest_magnitude(v, bits);
+			const float amax = clamped_amax(max_over_half_warp(bits));
+			store_codes<VEC>(y + offset, v, kLargestE4m3 / amax, column, l, limit);
+			if (l == 0 and b < blocks and inside)
+				scales[row * blocks + b] = amax / kLargestE4m3;
+		};
+		auto square_sum = [](const float (&v)[kPerLane], float sum)
+		{
+#pragma unroll
+			for (int i = 0; i < kPerLane; i++)
+				sum = fmaf(v[i], v[i], sum);
+			return sum;
+		};
+
+		constexpr int kHeld = ITEMS > 0 ? ITEMS : 1;
+		float v[kHeld][kPerLane];
+		float sum = 0.0f;
+		if constexpr (ITEMS > 0)
+		{
+#pragma unroll
+			for (int i = 0; i < kHeld; i++)
+				load_sum(v[i], (half + i * 2 * warps) * kScaleBlock);
+#pragma unroll
+			for (int i = 0; i < kHeld; i++)
+				sum = square_sum(v[i], sum);
+		}
+		else
+		{
+			for (int b = half; b < blocks; b += 2 * warps)
+			{
+				load_sum(v[0], b * kScaleBlock);
+				sum = square_sum(v[0], sum);
+			}
+			__syncwarp();
+		}
+#pragma unroll
+		for (int i = 16; i > 0; i /= 2)
+			sum += __shfl_xor_sync(kFullWarp, sum, i);
+		if (warps > 1)
+		{
+			if (threadIdx.x % 32 == 0)
+				warp_sum[warp] = sum;
+			__syncthreads();
+			sum = 0.0f;
+			for (int w = 0; w < warps; w++) /* the same order in every thread of the row */
+				sum += warp_sum[warp - warp_in_row + w];
+		}
+		const float rstd = 1.0f / sqrtf(sum / static_cast<float>(columns) + epsilon);
+		if constexpr (ITEMS > 0)
+		{
+#pragma unroll
+			for (int i = 0; i < kHeld; i++)
+				finish(v[i], half + i * 2 * warps, rstd);
+		}
+		else
+		{
+			/* both half-warps of a warp go round equally often: the maximum is taken with all lanes present */
+			for (int b = half; b - (half & 1) < blocks; b += 2 * warps)
+			{
+				load_sum(v[0], b * kScaleBlock);
+				finish(v[0], b, rstd);
+			}
+		}
+	}
+
+	int sm_count(const ContextObject &ctx)
+	{
+		int sms = 148;
+		cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx.device);
+		return sms;
+	}
+
+	template<typename T>
+	avStatus_t launch_quantize(ContextObject &ctx, const Operand &x, const Operand &y, const Operand &scales, long long rows, int columns, bool squares)
+	{
+		const int blocks = scale_blocks(columns);
+		const bool vec = columns % kPerLane == 0 and x.aligned(16) and y.aligned(8);
+		const T *xp = reinterpret_cast<const T*>(x.ptr);
+		float *sp = reinterpret_cast<float*>(scales.ptr);
+		cudaError_t launched;
+		if (squares)
+		{
+			const long long total = (rows + kScaleBlock - 1) / kScaleBlock * blocks;
+			const dim3 grid(static_cast<unsigned>(std::min<long long>(total, 1 << 30)));
+			auto kernel = vec ? kernel_quantize_squares<T, true> : kernel_quantize_squares<T, false>;
+			launched = launch_chained(kernel, grid, dim3(kThreads), 0, ctx.getStream(), xp, y.ptr, sp, total, rows, columns, blocks);
+		}
+		else
+		{
+			const long long total = rows * blocks;
+			const long long wanted = (total + kThreads / kLanes - 1) / (kThreads / kLanes);
+			const dim3 grid(static_cast<unsigned>(std::min<long long>(wanted, static_cast<long long>(sm_count(ctx)) * 8)));
+			auto kernel = vec ? kernel_quantize_rows<T, true> : kernel_quantize_rows<T, false>;
+			launched = launch_chained(kernel, grid, dim3(kThreads), 0, ctx.getStream(), xp, y.ptr, sp, total, columns, blocks);
+		}
+		return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
+	}
+
+	struct NormArgs
+	{
+			Operand x, z, h, gamma, y, scales;
+			long long rows;
+			int columns;
+			float epsilon;
+	};
+	template<typename T, bool VEC>
+	avStatus_t launch_norm(ContextObject &ctx, const NormArgs &a)
+	{
+		const int blocks = scale_blocks(a.columns);
+		/* Warps per row: enough that a half-warp holds at most four blocks; when the rows alone do not fill the machine, as many
+		 * as there are pairs of blocks, because then the time of one row is the time of the call. */
+		const bool few_rows = a.rows < 2 * sm_count(ctx);
+		const int wanted = few_rows ? (blocks + 1) / 2 : (blocks + 7) / 8;
+		int warps = 1;
+		while (warps < wanted and warps < 32)
+			warps *= 2;
+		const int per_half = (blocks + 2 * warps - 1) / (2 * warps);
+		const int threads = std::max(32 * warps, few_rows ? 32 : kThreads);
+		const long long rows_per_block = threads / (32 * warps);
+		const long long grid = (a.rows + rows_per_block - 1) / rows_per_block;
+		if (grid > 0x7FFFFFFFll)
+			return AVOCADO_STATUS_NOT_SUPPORTED;
+		auto kernel = per_half <= 1 ? kernel_rms_norm_quantize<T, 1, VEC> : per_half <= 2 ? kernel_rms_norm_quantize<T, 2, VEC> :
+				per_half <= 4 ? kernel_rms_norm_quantize<T, 4, VEC> : kernel_rms_norm_quantize<T, 0, VEC>;
+		const cudaError_t launched = launch_chained(kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, ctx.getStream(),
+				reinterpret_cast<const T*>(a.x.ptr), reinterpret_cast<const T*>(a.z.ptr), reinterpret_cast<T*>(a.h.ptr), reinterpret_cast<const float*>(a.gamma.ptr),
+				a.y.ptr, reinterpret_cast<float*>(a.scales.ptr), a.rows, a.columns, blocks, warps, a.epsilon);
+		return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
+	}
+	template<typename T>
+	avStatus_t launch_norm(ContextObject &ctx, const NormArgs &a)
+	{
+		const bool vec = a.columns % kPerLane == 0 and a.x.aligned(16) and a.z.aligned(16) and a.h.aligned(16) and a.gamma.aligned(16) and a.y.aligned(8);
+		return vec ? launch_norm<T, true>(ctx, a) : launch_norm<T, false>(ctx, a);
+	}
+
+	bool quantizable(avDataType_t dtype)
+	{
+		return dtype == AVOCADO_DTYPE_FLOAT16 or dtype == AVOCADO_DTYPE_BFLOAT16 or dtype == AVOCADO_DTYPE_FLOAT32;
+	}
+	bool same_shape(const TensorObject &a, const TensorObject &b)
+	{
+		if (a.nb_dims != b.nb_dims)
+			return false;
+		for (int i = 0; i < a.nb_dims; i++)
+			if (a.dims[i] != b.dims[i])
+				return false;
+		return true;
+	}
+}
+
+namespace avocado
+{
+	namespace backend
+	{
+		avStatus_t cudaQuantizeBlocks(avContextDescriptor_t context, const avTensorDescriptor_t xDesc, const avMemoryDescriptor_t xMem,
+				const avTensorDescriptor_t yDesc, avMemoryDescriptor_t yMem, const avTensorDescriptor_t scaleDesc, avMemoryDescriptor_t scaleMem)
+		{
+			AVOCADO_API_BEGIN
+				ContextObject &ctx = getContext(context);
+				const TensorObject &x = getTensor(xDesc);
+				const TensorObject &y = getTensor(yDesc);
+				const TensorObject &scale = getTensor(scaleDesc);
+				if (not quantizable(x.dtype) or y.dtype != AVOCADO_DTYPE_FLOAT8_E4M3 or scale.dtype != AVOCADO_DTYPE_FLOAT32)
+					return AVOCADO_STATUS_UNSUPPORTED_DATATYPE;
+				if (not valid_extents(x) or not valid_extents(scale) or not same_shape(x, y))
+					return AVOCADO_STATUS_BAD_PARAM;
+				const long long rows = row_count(x);
+				const int columns = x.lastDim();
+				const bool by_row = row_count(scale) == rows;
+				const bool squares = not by_row and row_count(scale) == (rows + kScaleBlock - 1) / kScaleBlock;
+				if (scale.lastDim() != scale_blocks(columns) or (not by_row and not squares))
+					return AVOCADO_STATUS_BAD_PARAM;
+				if (rows == 0 or columns == 0)
+					return AVOCADO_STATUS_SUCCESS;
+				if (columns > kMaxQuantizedRow)
+					return AVOCADO_STATUS_NOT_SUPPORTED;
+				Operand xo, yo, so;
+				if (not get_operand(xo, ctx, xMem, x) or not get_operand(yo, ctx, yMem, y) or not get_operand(so, ctx, scaleMem, scale))
+					return AVOCADO_STATUS_BAD_PARAM;
+				if (yo.overlaps(xo) or so.overlaps(xo) or so.overlaps(yo))
+					return AVOCADO_STATUS_BAD_PARAM;
+				ctx.setDevice();
+				switch (x.dtype)
+				{
+					case AVOCADO_DTYPE_FLOAT16:
+						return launch_quantize<half>(ctx, xo, yo, so, rows, columns, squares);
+					case AVOCADO_DTYPE_BFLOAT16:
+						return launch_quantize<__nv_bfloat16>(ctx, xo, yo, so, rows, columns, squares);
+					default:
+						return launch_quantize<float>(ctx, xo, yo, so, rows, columns, squares);
+				}
+			AVOCADO_API_END
+		}
+
+		avStatus_t cudaRmsNormQuantize(avContextDescriptor_t context, const avTensorDescriptor_t xDesc, const avMemoryDescriptor_t xMem,
+				const avMemoryDescriptor_t zMem, avMemoryDescriptor_t hMem, const avTensorDescriptor_t gammaDesc, const avMemoryDescriptor_t gammaMem,
+				double epsilon, const avTensorDescriptor_t yDesc, avMemoryDescriptor_t yMem, const avTensorDescriptor_t scaleDesc, avMemoryDescriptor_t scaleMem)
+		{
+			AVOCADO_API_BEGIN
+				ContextObject &ctx = getContext(context);
+				const TensorObject &x = getTensor(xDesc);
+				const TensorObject &gamma = getTensor(gammaDesc);
+				const TensorObject &y = getTensor(yDesc);
+				const TensorObject &scale = getTensor(scaleDesc);
+				if (not quantizable(x.dtype) or gamma.dtype != AVOCADO_DTYPE_FLOAT32 or y.dtype != AVOCADO_DTYPE_FLOAT8_E4M3 or scale.dtype != AVOCADO_DTYPE_FLOAT32)
+					return AVOCADO_STATUS_UNSUPPORTED_DATATYPE;
+				if (not valid_extents(x) or not valid_extents(scale) or not same_shape(x, y))
+					return AVOCADO_STATUS_BAD_PARAM;
+				NormArgs a;
+				a.rows = row_count(x);
+				a.columns = x.lastDim();
+				a.epsilon = static_cast<float>(epsilon);
+				if (gamma.nb_dims != 1 or gamma.dims[0] != a.columns or row_count(scale) != a.rows or scale.lastDim() != scale_blocks(a.columns))
+					return AVOCADO_STATUS_BAD_PARAM;
+				if (not (a.epsilon > 0.0f) or std::isinf(a.epsilon))
+					return AVOCADO_STATUS_BAD_PARAM;
+				if (a.rows == 0 or a.columns == 0)
+					return AVOCADO_STATUS_SUCCESS;
+				if (a.columns > kMaxNormedRow)
+					return AVOCADO_STATUS_NOT_SUPPORTED;
+				const bool has_z = zMem != AVOCADO_INVALID_DESCRIPTOR, has_h = hMem != AVOCADO_INVALID_DESCRIPTOR;
+				if (not get_operand(a.x, ctx, xMem, x) or (has_z and not get_operand(a.z, ctx, zMem, x)) or (has_h and not get_operand(a.h, ctx, hMem, x))
+						or not get_operand(a.gamma, ctx, gammaMem, gamma) or not get_operand(a.y, ctx, yMem, y)
+						or not get_operand(a.scales, ctx, scaleMem, scale))
+					return AVOCADO_STATUS_BAD_PARAM;
+				/* every thread writes h only where it has read x and z, so h may replace either of them, but not a shifted one */
+				if ((a.h.overlaps(a.x) and not a.h.same_as(a.x)) or (a.h.overlaps(a.z) and not a.h.same_as(a.z)) or a.h.overlaps(a.gamma))
+					return AVOCADO_STATUS_BAD_PARAM;
+				for (const Operand *out : { &a.y, &a.scales })
+					for (const Operand *other : { &a.x, &a.z, &a.h, &a.gamma })
+						if (out->overlaps(*other))
+							return AVOCADO_STATUS_BAD_PARAM;
+				if (a.y.overlaps(a.scales))
+					return AVOCADO_STATUS_BAD_PARAM;
+				ctx.setDevice();
+				switch (x.dtype)
+				{
+					case AVOCADO_DTYPE_FLOAT16:
+						return launch_norm<half>(ctx, a);
+					case AVOCADO_DTYPE_BFLOAT16:
+						return launch_norm<__nv_bfloat16>(ctx, a);
+					default:
+						return launch_norm<float>(ctx, a);
+				}
+			AVOCADO_API_END
+		}
+	} /* namespace backend */
+} /* namespace avocado */

@@ -71,7 +71,10 @@ namespace avocado
 			AVOCADO_DTYPE_FLOAT32,
 			AVOCADO_DTYPE_FLOAT64,
 			AVOCADO_DTYPE_COMPLEX32,
-			AVOCADO_DTYPE_COMPLEX64
+			AVOCADO_DTYPE_COMPLEX64,
+			/* 8-bit floating point: 4 exponent bits (bias 7), 3 mantissa bits, largest value 448, one NaN per sign, no infinity.
+			 * Not in the reference; taken by the block-scaled operators of cuda_backend_ext.h and by the calls that only move elements. */
+			AVOCADO_DTYPE_FLOAT8_E4M3
 		} avDataType_t;
 
 		typedef enum

@@ -117,6 +117,49 @@ DLL_PUBLIC avStatus_t cudaConvolutionWinogradFusedForwardNoAlloc(avContextDescri
 		const avTensorDescriptor_t bDesc, const avMemoryDescriptor_t bMem, const void *alpha2, const avTensorDescriptor_t zDesc,
 		const avMemoryDescriptor_t zMem, const void *beta, const avTensorDescriptor_t yDesc, avMemoryDescriptor_t yMem, avActivationType_t activation);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * 8-bit floating point with block scales: the quantised-inference path beside cudaGemm.  No counterpart in the reference.
+ *
+ * A quantised tensor is a pair: codes (AVOCADO_DTYPE_FLOAT8_E4M3) and float32 scales; a code q of a block with scale s stands
+ * for q * s.  Blocks lie along the last dimension, 128 elements each, the last one shorter when the extent is not a multiple
+ * of 128; the other dimensions are taken together as rows.  Two forms, told apart by the shape of the scales:
+ *   1 x 128    scales [rows..., ceil(C / 128)]              activations
+ *   128 x 128  scales [ceil(rows / 128), ceil(C / 128)]     weights
+ * With a = max(amax, 2^-100), amax being the largest magnitude in the block, the scale is a / 448 and the codes are
+ * round_to_nearest_even(x * (448 / a)), all in float32.  A block of zeros gets the scale of 2^-100 and zero codes.  A NaN
+ * makes its whole block NaN (scale and codes); an infinity gives an infinite scale, its own code NaN and zeros beside it.
+ *
+ * All three calls: memory blocks must hold at least what their descriptor says and lie on the context's device, and an output
+ * must not overlap an input or another output except where stated (AVOCADO_STATUS_BAD_PARAM otherwise).  No scratch memory is
+ * used and results do not depend on the order in which blocks run.  Tensors without elements succeed and write nothing.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/* x (float16, bfloat16, float32; any rank, rows of at most 2^30 elements) -> codes y (float8_e4m3, the shape of x) and scales,
+ * in the form that the shape of scaleDesc asks for. */
+DLL_PUBLIC avStatus_t cudaQuantizeBlocks(avContextDescriptor_t context, const avTensorDescriptor_t xDesc, const avMemoryDescriptor_t xMem,
+		const avTensorDescriptor_t yDesc, avMemoryDescriptor_t yMem, const avTensorDescriptor_t scaleDesc, avMemoryDescriptor_t scaleMem);
+
+/* Root-mean-square norm over the last dimension, with the residual's addition in front and the quantiser behind it, in one call:
+ *   h = x + z;   y = h / sqrt(mean(h^2) + epsilon) * gamma;   (codes, scales) = quantise(y) in 1 x 128 blocks
+ * x, z, h: float16, bfloat16 or float32, all of xDesc's type and shape, rows of at most 2^20 elements; gamma: float32 [C].  z is
+ * optional (AVOCADO_INVALID_DESCRIPTOR: h = x); h is rounded once into hMem when that is given, and may be stored over x or
+ * over z (the same memory, not a part of it).  Arithmetic is float32 and y is quantised without having been rounded before;
+ * squares overflow where |h| exceeds 1.8e19, as in any float32 norm.  epsilon must be positive and finite as a float32. */
+DLL_PUBLIC avStatus_t cudaRmsNormQuantize(avContextDescriptor_t context, const avTensorDescriptor_t xDesc, const avMemoryDescriptor_t xMem,
+		const avMemoryDescriptor_t zMem, avMemoryDescriptor_t hMem, const avTensorDescriptor_t gammaDesc, const avMemoryDescriptor_t gammaMem, double epsilon,
+		const avTensorDescriptor_t yDesc, avMemoryDescriptor_t yMem, const avTensorDescriptor_t scaleDesc, avMemoryDescriptor_t scaleMem);
+
+/* C = alpha * A * B^T + beta * C for quantised A [M, K] in 1 x 128 blocks and B [N, K] in 128 x 128 blocks:
+ *   C[m, n] = alpha * sum over g of aScale[m, g] * bScale[n / 128, g] * (sum over k in block g of A[m, k] * B[n, k]) + beta * C[m, n]
+ * aDesc, bDesc: float8_e4m3; scales float32 [M, ceil(K / 128)] and [ceil(N / 128), ceil(K / 128)]; C float16, bfloat16 or
+ * float32 [M, N]; alpha and beta float.  aOp must be N and bOp T (AVOCADO_STATUS_NOT_SUPPORTED otherwise).  Sums are float32,
+ * rounded once into C.  C is not read when beta is 0.  Row pitches of 16 bytes (K a multiple of 16, A and B on 16-byte
+ * boundaries) are copied by the tensor memory accelerator; other pitches are correct and slower. */
+DLL_PUBLIC avStatus_t cudaGemmBlockScaled(avContextDescriptor_t context, avGemmOperation_t aOp, avGemmOperation_t bOp, const void *alpha,
+		const avTensorDescriptor_t aDesc, const avMemoryDescriptor_t aMem, const avTensorDescriptor_t aScaleDesc, const avMemoryDescriptor_t aScaleMem,
+		const avTensorDescriptor_t bDesc, const avMemoryDescriptor_t bMem, const avTensorDescriptor_t bScaleDesc, const avMemoryDescriptor_t bScaleMem,
+		const void *beta, const avTensorDescriptor_t cDesc, avMemoryDescriptor_t cMem);
+
 #ifdef __cplusplus
 		} /* extern "C" */
 	} /* namespace backend */

@@ -319,3 +319,43 @@ def error_metrics(result, reference):
     norm = float(np.max(err) / max(float(np.max(np.abs(reference))), 1e-300)) if err.size else 0.0
     rms = float(np.sqrt(np.mean(err * err)) / rms_ref) if err.size else 0.0
     return {"elem": elem, "norm": norm, "rms": rms}
+
+
+def e4m3_round(v):
+    """Round to nearest, ties to even, onto the e4m3 grid (3 mantissa bits, exponents from -6); |v| <= 448 assumed."""
+    v = np.asarray(v, dtype=np.float64)
+    exponent = np.maximum(np.frexp(v)[1], -5)
+    step = np.ldexp(1.0, exponent - 4)
+    return np.rint(v / step) * step
+
+
+def block_scales(x, height=1):
+    """Scales of x[rows, C] in height x 128 blocks: max(amax, 2^-100) / 448 in float64."""
+    x = np.abs(_f64(x))
+    rows, c = x.shape
+    padded = np.zeros((-(-rows // height) * height, -(-c // 128) * 128))
+    padded[:rows, :c] = x
+    amax = padded.reshape(-1, height, padded.shape[1] // 128, 128).max(axis=(1, 3))
+    return np.maximum(amax, 2.0 ** -100) / 448.0
+
+
+def spread_scales(scales, rows, c, height=1):
+    """One scale per element of a [rows, C] matrix."""
+    return np.repeat(np.repeat(_f64(scales), height, axis=0)[:rows], 128, axis=1)[:, :c]
+
+
+def rms_norm(x, z, gamma, epsilon):
+    """(h, y): h = x + z, y = h / sqrt(mean(h^2) + epsilon) * gamma over the last dimension."""
+    h = _f64(x) + (0.0 if z is None else _f64(z))
+    return h, h / np.sqrt(np.mean(h * h, axis=-1, keepdims=True) + epsilon) * _f64(gamma)
+
+
+def gemm_block_scaled(a, a_scale, b, b_scale, alpha=1.0, beta=0.0, c=None):
+    """alpha * (a * a_scale) (b * b_scale)^T + beta * c for a[M, K] in 1 x 128 and b[N, K] in 128 x 128 blocks, and the sum of
+    the magnitudes of its terms (what rounding errors are measured by)."""
+    a = _f64(a) * spread_scales(a_scale, *np.shape(a))
+    b = _f64(b) * spread_scales(b_scale, *np.shape(b), 128)
+    out, size = alpha * (a @ b.T), abs(alpha) * (np.abs(a) @ np.abs(b).T)
+    if c is not None and beta != 0.0:
+        out, size = out + beta * _f64(c), size + abs(beta) * np.abs(_f64(c))
+    return out, size

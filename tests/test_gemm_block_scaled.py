@@ -1,0 +1,225 @@
+"""cudaGemmBlockScaled against the formula in float64."""
+import numpy as np
+import pytest
+
+from cudabackend_b200 import api
+from oracle import oracle as o
+from tests import block_scaled as bs
+
+pytestmark = pytest.mark.gpu
+
+# (M, N, K): one token and small batches, tile edges on both sides, short last blocks of K, several tiles and blocks of every kernel
+SHAPES = [(1, 1, 16), (1, 128, 128), (1, 257, 384), (2, 64, 16), (7, 130, 144), (1, 4096, 2048), (16, 128, 1008), (17, 129, 256), (33, 200, 2048),
+          (64, 512, 640), (65, 384, 128), (128, 128, 4096), (129, 127, 112), (130, 513, 272), (255, 256, 512), (300, 520, 1040), (1000, 264, 2304),
+          (257, 512, 128), (513, 1024, 384), (2100, 1300, 1280), (4100, 256, 576), (3000, 2056, 272)]
+# row pitches that are no multiple of 16 bytes
+ODD_SHAPES = [(1, 1, 1), (1, 300, 77), (5, 70, 33), (64, 64, 7), (130, 140, 129), (200, 300, 517), (33, 257, 260), (300, 129, 1002), (513, 520, 264), (1, 1024, 4095)]
+
+
+class Problem:
+    def __init__(self, ctx, m, n, k, dtype, seed=91, a_offset=0, b_offset=0, c_offset=0, c_values=None):
+        r = np.random.default_rng(seed)
+        self.ctx, self.k, self.dtype = ctx, k, dtype
+        self.a = bs.Placed(ctx, (m, k), "float8_e4m3", a_offset, bs.random_codes(r, m, k))
+        self.b = bs.Placed(ctx, (n, k), "float8_e4m3", b_offset, bs.random_codes(r, n, k))
+        # scales over several powers of two, so that one applied to the wrong block shows
+        self.sa = bs.Placed(ctx, (m, bs.blocks(k)), "float32", 4, np.exp2(r.uniform(-9, -3, (m, bs.blocks(k)))))
+        self.sb = bs.Placed(ctx, (bs.blocks(n), bs.blocks(k)), "float32", 8, np.exp2(r.uniform(-9, -3, (bs.blocks(n), bs.blocks(k)))))
+        self.c = bs.Placed(ctx, (m, n), dtype, c_offset, r.normal(0, 1, (m, n)) if c_values is None else c_values)
+
+    def run(self, alpha=None, beta=None):
+        bs.gemm(self.ctx, self.a, self.sa, self.b, self.sb, self.c, alpha, beta)
+
+    def expected(self, alpha=1.0, beta=0.0):
+        f = lambda v: float(np.float32(v))
+        return o.gemm_block_scaled(self.a.values, self.sa.values, self.b.values, self.sb.values, f(alpha), f(beta), self.c.values)
+
+    def check(self, alpha=1.0, beta=0.0):
+        ref, size = self.expected(alpha, beta)
+        got = self.c.download()
+        assert np.all(np.abs(got - ref) <= bs.gemm_error_bound(ref, size, self.k, self.dtype))
+        assert self.c.guards_intact()
+        return got
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_products(ctx, dtype, shape):
+    p = Problem(ctx, *shape, dtype)
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("shape", ODD_SHAPES)
+def test_odd_row_pitches(ctx, dtype, shape):
+    p = Problem(ctx, *shape, dtype)
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("a_offset,b_offset,c_offset", [(1, 0, 0), (0, 2, 0), (4, 4, 0), (8, 0, 2), (0, 8, 4), (0, 0, 2), (0, 0, 8), (16, 32, 16)])
+@pytest.mark.parametrize("shape", [(3, 264, 256), (140, 300, 272), (600, 512, 256)])
+def test_unaligned_views(ctx, a_offset, b_offset, c_offset, shape):
+    p = Problem(ctx, *shape, "bfloat16", a_offset=a_offset, b_offset=b_offset, c_offset=c_offset)
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("shape", [(1, 300, 256), (40, 128, 384), (100, 300, 1000), (130, 257, 528), (1111, 1032, 640), (1000, 300, 77)])
+def test_small_integers_are_exact(ctx, shape):
+    """codes that are integers up to 8 and scales that are powers of two: every partial sum is a float32 number, whatever the order"""
+    m, n, k = shape
+    p = Problem(ctx, m, n, k, "float32")
+    r = np.random.default_rng(92)
+    p.a.upload(r.integers(-8, 9, (m, k)))
+    p.b.upload(r.integers(-8, 9, (n, k)))
+    p.sa.upload(np.exp2(r.integers(-2, 2, (m, bs.blocks(k)))))
+    p.sb.upload(np.exp2(r.integers(-2, 2, (bs.blocks(n), bs.blocks(k)))))
+    p.run()
+    assert np.array_equal(p.c.download(), p.expected()[0])
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("shape", [(5, 136, 272), (200, 300, 512), (700, 520, 256), (33, 130, 77)])
+def test_alpha_and_beta(ctx, dtype, shape):
+    p = Problem(ctx, *shape, dtype)
+    p.run(0.37, -1.25)
+    p.check(0.37, -1.25)
+
+
+@pytest.mark.parametrize("shape", [(3, 256, 256), (130, 128, 128), (600, 300, 256)])
+def test_c_is_not_read_without_beta(ctx, shape):
+    m, n, _ = shape
+    p = Problem(ctx, *shape, "float32", c_values=np.full((m, n), np.nan))
+    p.run(2.0, 0.0)
+    ref, size = o.gemm_block_scaled(p.a.values, p.sa.values, p.b.values, p.sb.values, 2.0)
+    assert np.all(np.abs(p.c.download() - ref) <= bs.gemm_error_bound(ref, size, p.k, "float32"))
+
+
+@pytest.mark.parametrize("shape", [(20, 300, 384), (150, 300, 384), (600, 512, 384)])
+def test_nan_and_infinity_stay_in_their_rows(ctx, shape):
+    m, n, k = shape
+    p = Problem(ctx, m, n, k, "float32")
+    a = p.a.values.copy()
+    a[3, 200] = np.nan
+    p.a.upload(a)
+    sa = p.sa.values.copy()
+    sa[7, 2], sa[11, 0] = np.nan, np.inf
+    p.sa.upload(sa)
+    p.run()
+    got = p.c.download()
+    assert np.all(np.isnan(got[[3, 7]])) and not np.any(np.isfinite(got[11]))
+    keep = np.setdiff1d(np.arange(m), [3, 7, 11])
+    ref, size = o.gemm_block_scaled(p.a.values[keep], p.sa.values[keep], p.b.values, p.sb.values)
+    assert np.all(np.abs(got[keep] - ref) <= bs.gemm_error_bound(ref, size, k, "float32"))
+
+
+@pytest.mark.parametrize("shape", [(16, 4096, 4096), (100, 520, 2048), (2000, 1032, 1024), (65, 200, 999)])
+def test_same_bits_every_time(ctx, shape):
+    p = Problem(ctx, *shape, "float32")
+    p.run()
+    first = p.c.raw().copy()
+    for _ in range(3):
+        p.run()
+        assert np.array_equal(first.view(np.uint32), p.c.raw().view(np.uint32))
+
+
+def test_rows_do_not_depend_on_the_batch_they_are_in_within_a_kernel(ctx):
+    """rows 0..7 of a batch of 8 and of 13: the same kernel and split, so the same bits"""
+    p = Problem(ctx, 13, 1024, 2048, "float32")
+    p.run()
+    whole = p.c.download()
+    q = Problem(ctx, 8, 1024, 2048, "float32")
+    q.a.upload(p.a.values[:8])
+    q.sa.upload(p.sa.values[:8])
+    q.b.upload(p.b.values)
+    q.sb.upload(p.sb.values)
+    q.run()
+    assert np.array_equal(q.c.download(), whole[:8])
+
+
+@pytest.mark.parametrize("shape", [(0, 5, 128), (5, 0, 128)])
+def test_no_rows_or_columns(ctx, shape):
+    m, n, k = shape
+    a, b, c = bs.Placed(ctx, (m, k), "float8_e4m3"), bs.Placed(ctx, (n, k), "float8_e4m3"), bs.Placed(ctx, (m, n), "float32")
+    sa, sb = bs.Placed(ctx, (m, 1), "float32"), bs.Placed(ctx, (bs.blocks(n), 1), "float32")
+    bs.gemm(ctx, a, sa, b, sb, c)
+    assert c.guards_intact()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 5), (300, 257)])
+def test_an_empty_sum(ctx, dtype, shape):
+    """K = 0: C = beta * C"""
+    m, n = shape
+    a, b, c = bs.Placed(ctx, (m, 0), "float8_e4m3"), bs.Placed(ctx, (n, 0), "float8_e4m3"), bs.Placed(ctx, (m, n), dtype, values=np.full((m, n), 3.0))
+    sa, sb = bs.Placed(ctx, (m, 0), "float32"), bs.Placed(ctx, (bs.blocks(n), 0), "float32")
+    bs.gemm(ctx, a, sa, b, sb, c, beta=0.5)
+    assert np.all(c.download() == 1.5) and c.guards_intact()
+    bs.gemm(ctx, a, sa, b, sb, c)
+    assert np.all(c.download() == 0.0) and c.guards_intact()
+
+
+def test_refusals(ctx):
+    P = bs.Placed
+    base = {"a": P(ctx, (40, 300), "float8_e4m3"), "a_scale": P(ctx, (40, 3), "float32"), "b": P(ctx, (200, 300), "float8_e4m3"),
+            "b_scale": P(ctx, (2, 3), "float32"), "c": P(ctx, (40, 200), "bfloat16")}
+    for name in ("a", "b", "a_scale", "b_scale"):
+        base[name].upload(np.zeros(base[name].shape))
+
+    def status(**change):
+        return bs.gemm(ctx, status=True, **{**base, **change})
+
+    bad, dtype = api.STATUS["BAD_PARAM"], api.STATUS["UNSUPPORTED_DATATYPE"]
+    assert status() == api.STATUS["SUCCESS"]
+    for ops in ((0, 0), (1, 1), (1, 0)):
+        assert status(ops=ops) == api.STATUS["NOT_SUPPORTED"]
+    assert status(a=P(ctx, (40, 300), "int8")) == dtype and status(b=P(ctx, (200, 300), "bfloat16")) == dtype
+    assert status(c=P(ctx, (40, 200), "float64")) == dtype and status(c=P(ctx, (40, 200), "int32")) == dtype
+    assert status(a_scale=P(ctx, (40, 3), "float16")) == dtype and status(b_scale=P(ctx, (2, 3), "float64")) == dtype
+    assert status(a=P(ctx, (40, 299), "float8_e4m3")) == bad and status(b=P(ctx, (200, 301), "float8_e4m3")) == bad
+    assert status(c=P(ctx, (200, 40), "bfloat16")) == bad and status(c=P(ctx, (1, 40, 200), "bfloat16")) == bad
+    for shape in ((40, 2), (1, 3), (120,), (3, 40)):
+        assert status(a_scale=P(ctx, shape, "float32")) == bad, shape
+    for shape in ((200, 3), (2, 2), (1, 3), (3, 2)):
+        assert status(b_scale=P(ctx, shape, "float32")) == bad, shape
+    short = P(ctx, (200, 300), "float8_e4m3")
+    short.mem = short.block.view(200 * 300 - 1, 0)
+    assert status(b=short) == bad
+    over = P(ctx, (40, 200), "bfloat16")
+    over.mem = base["b"].block.view(40 * 200 * 2, 100)
+    assert status(c=over) == bad
+    off = P(ctx, (40, 200), "bfloat16")
+    off.mem = off.block.view(40 * 200 * 2, 1)
+    assert status(c=off) == bad
+    huge = P(ctx, (1, 1), "float8_e4m3")
+    api.call("cudaSetTensorDescriptor", huge.desc.handle, api.DTYPES["float8_e4m3"], 2, (api._INT * 2)(2 ** 31 - 1, 2 ** 31 - 1))
+    assert status(a=huge) == bad
+    assert base["c"].guards_intact()
+
+
+@pytest.mark.parametrize("n,k", [(2056, 2048), (4, 2050)])
+def test_offsets_past_32_bits(ctx, n, k):
+    """A of more than 2^31 bytes and, in the first case, C of more than 2^31 elements (2^32 bytes)"""
+    m = 1100003
+    a_desc, c_desc = api.TensorDescriptor((m, k), "float8_e4m3"), api.TensorDescriptor((m, n), "bfloat16")
+    sa_desc = api.TensorDescriptor((m, bs.blocks(k)), "float32")
+    a, c, sa = api.Memory(a_desc.nbytes), api.Memory(c_desc.nbytes), api.Memory(sa_desc.nbytes)
+    a.zero(ctx), sa.zero(ctx)
+    r = np.random.default_rng(93)
+    keep = 64
+    codes, a64 = api.to_storage(bs.random_codes(r, keep, k), "float8_e4m3")
+    scales, sa64 = api.to_storage(np.exp2(r.uniform(-9, -3, (keep, bs.blocks(k)))), "float32")
+    for first in (0, m - keep):
+        a.from_host(ctx, codes, first * k)
+        sa.from_host(ctx, scales, first * bs.blocks(k) * 4)
+    b = bs.Placed(ctx, (n, k), "float8_e4m3", values=bs.random_codes(r, n, k))
+    sb = bs.Placed(ctx, (bs.blocks(n), bs.blocks(k)), "float32", values=np.exp2(r.uniform(-9, -3, (bs.blocks(n), bs.blocks(k)))))
+    api.call("cudaGemmBlockScaled", ctx.handle, api.GEMM_N, api.GEMM_T, None, a_desc.handle, a.handle, sa_desc.handle, sa.handle, b.desc.handle, b.mem.handle,
+             sb.desc.handle, sb.mem.handle, None, c_desc.handle, c.handle)
+    ref, size = o.gemm_block_scaled(a64, sa64, b.values, sb.values)
+    for first in (0, m - keep):
+        got = c.to_host(ctx, np.empty((keep, n), dtype=np.uint16), first * n * 2)
+        ctx.synchronize()
+        assert np.all(np.abs(api.bfloat16_bits_to_float(got) - ref) <= bs.gemm_error_bound(ref, size, k, "bfloat16"))
