@@ -12,8 +12,6 @@
 #include "objects.hpp"
 #include "umma.cuh"
 
-#include <cuda_fp8.h>
-
 #include <algorithm>
 
 namespace
@@ -21,6 +19,9 @@ namespace
 	using namespace avocado::backend;
 	using namespace avocado::backend::b200;
 	using namespace bk;
+
+	constexpr int kBlockBytes = 128 * kScaleBlock; /* one operand tile: 128 rows of one block of K */
+	constexpr int kMaxSplits = 8;                  /* CTAs of a cluster, the portable limit */
 
 	struct ScaledGemm
 	{
@@ -30,71 +31,504 @@ namespace
 			const float *a_scale, *b_scale;
 			void *c;
 			float alpha, beta;
+			int c_type; /* avDataType_t of C */
+			int c_vector; /* four neighbouring elements of C can be moved at once */
 	};
 
-	/* Plain form on the CUDA cores: a block computes 64 x 64 results, 16 per thread, from 32 elements of K at a time. */
-	template<typename T>
-	__global__ void __launch_bounds__(256) kernel_gemm_f8_simt(ScaledGemm p)
+	/* ---- C in any of its three types ------------------------------------------------------------------------------ */
+	__device__ __forceinline__ float load_c(const ScaledGemm &p, long long i)
 	{
-		constexpr int kTile = 64, kStep = 32;
-		__shared__ float a_s[kStep][kTile + 1], b_s[kStep][kTile + 1];
-		chain_release();
-		chain_wait();
-		const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-		const long long tiles_n = (p.N + kTile - 1) / kTile;
-		const long long m0 = blockIdx.x / tiles_n * kTile, n0 = blockIdx.x % tiles_n * kTile;
-		float acc[4][4] = { };
-		for (int g = 0; g < p.blocks; g++)
+		if (p.c_type == AVOCADO_DTYPE_FLOAT32)
+			return reinterpret_cast<const float*>(p.c)[i];
+		if (p.c_type == AVOCADO_DTYPE_FLOAT16)
+			return to_compute(reinterpret_cast<const half*>(p.c)[i]);
+		return to_compute(reinterpret_cast<const __nv_bfloat16*>(p.c)[i]);
+	}
+	__device__ __forceinline__ void store_c(const ScaledGemm &p, long long i, float v)
+	{
+		if (p.c_type == AVOCADO_DTYPE_FLOAT32)
+			reinterpret_cast<float*>(p.c)[i] = v;
+		else if (p.c_type == AVOCADO_DTYPE_FLOAT16)
+			reinterpret_cast<half*>(p.c)[i] = from_compute<half>(v);
+		else
+			reinterpret_cast<__nv_bfloat16*>(p.c)[i] = from_compute<__nv_bfloat16>(v);
+	}
+	__device__ __forceinline__ uint32_t pack_two(int c_type, float x, float y)
+	{
+		if (c_type == AVOCADO_DTYPE_FLOAT16)
 		{
-			float part[4][4] = { };
-			for (int k0 = g * kScaleBlock; k0 < min(p.K, (g + 1) * kScaleBlock); k0 += kStep)
-			{
-				for (int i = threadIdx.x; i < kTile * kStep; i += 256)
-				{
-					const int r = i / kStep, k = i % kStep;
-					__nv_fp8_e4m3 va, vb;
-					va.__x = (m0 + r < p.M and k0 + k < p.K) ? p.a[(m0 + r) * p.K + k0 + k] : 0;
-					vb.__x = (n0 + r < p.N and k0 + k < p.K) ? p.b[(n0 + r) * p.K + k0 + k] : 0;
-					a_s[k][r] = static_cast<float>(va);
-					b_s[k][r] = static_cast<float>(vb);
-				}
-				__syncthreads();
-				for (int k = 0; k < kStep; k++)
-					for (int i = 0; i < 4; i++)
-						for (int j = 0; j < 4; j++)
-							part[i][j] = fmaf(a_s[k][ty * 4 + i], b_s[k][tx + j * 16], part[i][j]);
-				__syncthreads();
-			}
-			for (int i = 0; i < 4; i++)
-			{
-				const long long m = m0 + ty * 4 + i;
-				const float sa = m < p.M ? p.a_scale[m * p.blocks + g] : 0.0f;
-				const float s = sa * p.b_scale[n0 / kScaleBlock * p.blocks + g];
-				for (int j = 0; j < 4; j++)
-					acc[i][j] = fmaf(part[i][j], s, acc[i][j]);
-			}
+			const half2 v = __floats2half2_rn(x, y);
+			return *reinterpret_cast<const uint32_t*>(&v);
 		}
-		T *c = reinterpret_cast<T*>(p.c);
-		for (int i = 0; i < 4; i++)
+		const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+		return *reinterpret_cast<const uint32_t*>(&v);
+	}
+	/* alpha * v + beta * C for four neighbouring elements of a row, of which `count` exist */
+	__device__ __forceinline__ void finish_four(const ScaledGemm &p, long long i, float4 v, int count)
+	{
+		float x[4] = { p.alpha * v.x, p.alpha * v.y, p.alpha * v.z, p.alpha * v.w };
+		if (p.beta != 0.0f)
+		{
+#pragma unroll
 			for (int j = 0; j < 4; j++)
-			{
-				const long long m = m0 + ty * 4 + i, n = n0 + tx + j * 16;
-				if (m < p.M and n < p.N)
-				{
-					const float old = p.beta != 0.0f ? p.beta * to_compute(c[m * p.N + n]) : 0.0f;
-					c[m * p.N + n] = from_compute<T>(fmaf(p.alpha, acc[i][j], old));
-				}
-			}
+				if (j < count)
+					x[j] = fmaf(p.beta, load_c(p, i + j), x[j]);
+		}
+		if (p.c_vector)
+		{
+			if (p.c_type == AVOCADO_DTYPE_FLOAT32)
+				*reinterpret_cast<float4*>(reinterpret_cast<float*>(p.c) + i) = make_float4(x[0], x[1], x[2], x[3]);
+			else
+				*reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.c) + i) = make_uint2(pack_two(p.c_type, x[0], x[1]), pack_two(p.c_type, x[2], x[3]));
+		}
+		else
+		{
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				if (j < count)
+					store_c(p, i + j, x[j]);
+		}
 	}
 
-	template<typename T>
+	/* K = 0: the sum is empty */
+	__global__ void __launch_bounds__(256) kernel_scale_c(ScaledGemm p)
+	{
+		chain_release();
+		chain_wait();
+		const long long total = static_cast<long long>(p.M) * p.N;
+		for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * 256)
+			store_c(p, i, p.beta != 0.0f ? p.beta * load_c(p, i) : 0.0f);
+	}
+
+	/*
+	 * Few rows of A ("tokens"), and any row pitch: 128 rows of B are the M side of the MMA and TOKENS rows of A its N side, so
+	 * that a handful of tokens does not waste 128-row tiles; the result is transposed on the way out.
+	 *
+	 * Bound: the bytes of B.  One tile of 128 rows of B per CTA leaves most SMs without work at the usual sizes, so the blocks of
+	 * K are split over the CTAs of a cluster; their partial sums meet in distributed shared memory and are added in the order
+	 * of the ranks (no scratch memory, no atomics, the same bits every time).
+	 *
+	 * One ring of STAGES slots serves three roles: full (copy -> MMA), done (MMA -> promotion), drained (promotion -> copy).  Each
+	 * block of K has its own accumulator in TMEM, because its scales are applied outside the tensor core:
+	 * acc[t] += scale[t] * part[t] in float32 registers, thread = row of B.  PER_STAGE blocks share a slot, so that the thread
+	 * that issues the MMAs waits and commits once per PER_STAGE * 4 MMAs.
+	 *
+	 * LOADERS: four warps fill the slots with plain loads instead of the TMA copies, for row pitches or addresses that are no
+	 * multiple of 16 bytes.
+	 */
+	template<int TOKENS, bool LOADERS>
+	struct SplitConfig
+	{
+			static constexpr int kPerStage = TOKENS <= 64 ? 2 : 1;
+			static constexpr int kStages = 4;
+			static constexpr int kPairBytes = kBlockBytes + TOKENS * kScaleBlock;
+			static constexpr int kStageBytes = kPerStage * kPairBytes;
+			/* Two CTAs of different clusters never share an SM: each could wait for the TMEM of the other's neighbour. */
+			static constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+			static_assert(kSmemBytes > 116 * 1024 and kSmemBytes <= 228 * 1024, "one CTA per SM");
+			static_assert(TOKENS * 512 <= kStages * kStageBytes, "the partial sums reuse the slots");
+			static constexpr int kWantedColumns = kStages * kPerStage * TOKENS;
+			static constexpr int kTmemColumns = kWantedColumns <= 128 ? 128 : kWantedColumns <= 256 ? 256 : 512;
+			static constexpr int kLoaderThreads = LOADERS ? 128 : 32;
+			static constexpr int kThreads = 160 + kLoaderThreads;
+	};
+
+	/* 16 bytes from any address, zero past the first `valid`; only bytes inside [low, high) are touched */
+	__device__ __forceinline__ uint4 load_unaligned(const uint8_t *ptr, int valid, const uint8_t *low, const uint8_t *high)
+	{
+		uint32_t w[5];
+		const int offset = static_cast<int>(reinterpret_cast<uintptr_t>(ptr) & 3);
+		const uint8_t *base = ptr - offset;
+#pragma unroll
+		for (int i = 0; i < 5; i++)
+		{
+			const uint8_t *at = base + 4 * i;
+			w[i] = 0;
+			if (4 * i < offset + valid)
+			{
+				if (at >= low and at + 4 <= high)
+					w[i] = *reinterpret_cast<const uint32_t*>(at);
+				else
+					for (int j = 0; j < 4; j++)
+						if (at + j >= low and at + j < high)
+							w[i] |= static_cast<uint32_t>(at[j]) << (8 * j);
+			}
+		}
+		uint32_t r[4];
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+		{
+			r[i] = __funnelshift_r(w[i], w[i + 1], 8 * offset);
+			const int left = valid - 4 * i;
+			if (left < 4)
+				r[i] = left <= 0 ? 0u : r[i] & ((1u << (8 * left)) - 1u);
+		}
+		return make_uint4(r[0], r[1], r[2], r[3]);
+	}
+
+	template<int TOKENS, bool LOADERS>
+	__global__ void __launch_bounds__(SplitConfig<TOKENS, LOADERS>::kThreads, 1) kernel_gemm_f8_split(const __grid_constant__ CUtensorMap mapA,
+			const __grid_constant__ CUtensorMap mapB, ScaledGemm p, int tokenTiles, int splits, int blocksPerSplit, int *deviceStatus)
+	{
+		using Cfg = SplitConfig<TOKENS, LOADERS>;
+		constexpr int kStages = Cfg::kStages, kPerStage = Cfg::kPerStage;
+		extern __shared__ uint8_t smem_raw[];
+		uint8_t *smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+
+		__shared__ __align__(8) uint64_t full_bar[kStages];
+		__shared__ __align__(8) uint64_t done_bar[kStages];
+		__shared__ __align__(8) uint64_t drained_bar[kStages];
+		__shared__ uint32_t tmem_base_slot;
+		__shared__ int abort_flag;
+		__shared__ __align__(16) float scale_s[4][kPerStage * TOKENS];
+
+		const int warp = threadIdx.x / 32;
+		const int lane = threadIdx.x % 32;
+		const int rank = splits > 1 ? static_cast<int>(umma::cluster_cta_rank()) : 0;
+		const int tile = blockIdx.x / splits;
+		const int m0 = tile % tokenTiles * TOKENS;
+		const int n_block = tile / tokenTiles;
+		const int n0 = n_block * 128;
+		const int first = min(p.blocks, rank * blocksPerSplit);
+		const int last = min(p.blocks, first + blocksPerSplit);
+
+		if (threadIdx.x == 0)
+		{
+			abort_flag = 0;
+			for (int s = 0; s < kStages; s++)
+			{
+				umma::mbar_init(&full_bar[s], LOADERS ? Cfg::kLoaderThreads : 1);
+				umma::mbar_init(&done_bar[s], 1);
+				umma::mbar_init(&drained_bar[s], 4);
+			}
+			umma::mbar_fence_init();
+			if (not LOADERS)
+			{
+				umma::prefetch_tensormap(&mapA);
+				umma::prefetch_tensormap(&mapB);
+			}
+		}
+		if (warp == 4)
+		{
+			umma::tmem_alloc(&tmem_base_slot, Cfg::kTmemColumns);
+			umma::tmem_relinquish();
+		}
+		umma::tcgen05_fence_before();
+		__syncthreads();
+		umma::tcgen05_fence_after();
+		const uint32_t tmem_base = tmem_base_slot;
+		volatile int *abort_ptr = &abort_flag;
+		chain_release();
+		chain_wait();
+
+		if (warp == 4)
+		{
+			if (lane == 0)
+			{
+				constexpr uint32_t idesc = umma::make_instr_desc(umma::kAccumF32, umma::kFormatE4M3, umma::kFormatE4M3, false, false, 128, TOKENS);
+				const uint64_t desc0 = umma::make_smem_desc(umma::smem_u32(smem), 16, 1024, umma::kSwizzle128B);
+				int stage = 0;
+				uint32_t phase = 0;
+				for (int kb = first; kb < last; kb += kPerStage)
+				{
+					if (not umma::mbar_wait(&full_bar[stage], phase, abort_ptr))
+					{
+						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorTmaWait);
+						break;
+					}
+					umma::tcgen05_fence_after();
+#pragma unroll
+					for (int j = 0; j < kPerStage; j++)
+						if (kb + j < last)
+						{
+							const uint64_t desc = desc0 + static_cast<uint64_t>((stage * Cfg::kStageBytes + j * Cfg::kPairBytes) / 16);
+							umma::mma_f8_k4(tmem_base + static_cast<uint32_t>((stage * kPerStage + j) * TOKENS), desc, desc + kBlockBytes / 16, idesc, false);
+						}
+					umma::mma_commit(&done_bar[stage]);
+					if (++stage == kStages)
+					{
+						stage = 0;
+						phase ^= 1u;
+					}
+				}
+			}
+		}
+		else if (warp > 4)
+		{
+			if (LOADERS or lane == 0)
+			{
+				const int thread = threadIdx.x - 160;
+				int stage = 0;
+				uint32_t phase = 0;
+				for (int kb = first; kb < last; kb += kPerStage)
+				{
+					const int count = min(kPerStage, last - kb);
+					if (not umma::mbar_wait(&drained_bar[stage], phase ^ 1u, abort_ptr))
+					{
+						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorStageWait);
+						break;
+					}
+					uint8_t *slot = smem + stage * Cfg::kStageBytes;
+					if constexpr (LOADERS)
+					{
+						/* piece i of a row lies at piece i ^ (row % 8): the 128-byte swizzle that the descriptors name */
+						for (int j = 0; j < count; j++)
+						{
+							const int k = (kb + j) * kScaleBlock + thread % 8 * 16;
+							const int valid = max(0, min(16, p.K - k));
+#pragma unroll 4
+							for (int row = thread / 8; row < 128 + TOKENS; row += Cfg::kLoaderThreads / 8)
+							{
+								const bool weights = row < 128;
+								const int r = weights ? row : row - 128;
+								const long long global = weights ? n0 + static_cast<long long>(r) : m0 + static_cast<long long>(r);
+								const long long rows = weights ? p.N : p.M;
+								const uint8_t *base = weights ? p.b : p.a;
+								uint4 v = make_uint4(0, 0, 0, 0);
+								if (global < rows and valid > 0)
+									v = load_unaligned(base + global * p.K + k, valid, base, base + rows * p.K);
+								*reinterpret_cast<uint4*>(slot + j * Cfg::kPairBytes + (weights ? 0 : kBlockBytes) + r * 128 + ((thread % 8) ^ (r & 7)) * 16) = v;
+							}
+						}
+						umma::fence_proxy_async_smem();
+						umma::mbar_arrive(&full_bar[stage]);
+					}
+					else
+					{
+						umma::mbar_arrive_expect_tx(&full_bar[stage], static_cast<uint32_t>(count * Cfg::kPairBytes));
+						for (int j = 0; j < count; j++)
+						{
+							umma::tma_load_2d(slot + j * Cfg::kPairBytes, &mapB, &full_bar[stage], (kb + j) * kScaleBlock, n0);
+							umma::tma_load_2d(slot + j * Cfg::kPairBytes + kBlockBytes, &mapA, &full_bar[stage], (kb + j) * kScaleBlock, m0);
+						}
+					}
+					if (++stage == kStages)
+					{
+						stage = 0;
+						phase ^= 1u;
+					}
+				}
+			}
+		}
+		else
+		{
+			/* promotion: thread = row n0 + threadIdx.x of B, one accumulator per token */
+			float acc[TOKENS];
+#pragma unroll
+			for (int t = 0; t < TOKENS; t++)
+				acc[t] = 0.0f;
+			constexpr int kScales = kPerStage * TOKENS / 32; /* scales of a slot per lane */
+			float next[kScales];
+			auto fetch = [&](int kb)
+			{
+#pragma unroll
+				for (int i = 0; i < kScales; i++)
+				{
+					const int t = (i * 32 + lane) % TOKENS, g = kb + (i * 32 + lane) / TOKENS;
+					next[i] = 0.0f;
+					if (g < last and m0 + t < p.M)
+						next[i] = p.a_scale[static_cast<long long>(m0 + t) * p.blocks + g] * p.b_scale[static_cast<long long>(n_block) * p.blocks + g];
+				}
+			};
+			fetch(first);
+			const uint32_t lanes = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+			int stage = 0;
+			uint32_t phase = 0;
+			bool ok = true;
+			for (int kb = first; kb < last; kb += kPerStage)
+			{
+				__syncwarp(); /* the scales of the slot before have been read */
+#pragma unroll
+				for (int i = 0; i < kScales; i++)
+					scale_s[warp][i * 32 + lane] = next[i];
+				__syncwarp();
+				fetch(kb + kPerStage);
+				ok = __all_sync(0xFFFFFFFFu, umma::mbar_wait(&done_bar[stage], phase, abort_ptr));
+				if (not ok)
+				{
+					if (lane == 0)
+						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
+					break;
+				}
+				umma::tcgen05_fence_after();
+#pragma unroll
+				for (int j = 0; j < kPerStage; j++)
+				{
+					if (kb + j >= last)
+						break;
+#pragma unroll
+					for (int t0 = 0; t0 < TOKENS; t0 += 16)
+					{
+						uint32_t r[16];
+						umma::tmem_load_32x16(lanes + static_cast<uint32_t>((stage * kPerStage + j) * TOKENS + t0), r);
+						umma::tmem_load_wait();
+#pragma unroll
+						for (int t = 0; t < 16; t += 4)
+						{
+							const float4 s = *reinterpret_cast<const float4*>(&scale_s[warp][j * TOKENS + t0 + t]);
+							acc[t0 + t] = fmaf(__uint_as_float(r[t]), s.x, acc[t0 + t]);
+							acc[t0 + t + 1] = fmaf(__uint_as_float(r[t + 1]), s.y, acc[t0 + t + 1]);
+							acc[t0 + t + 2] = fmaf(__uint_as_float(r[t + 2]), s.z, acc[t0 + t + 2]);
+							acc[t0 + t + 3] = fmaf(__uint_as_float(r[t + 3]), s.w, acc[t0 + t + 3]);
+						}
+					}
+				}
+				umma::tcgen05_fence_before();
+				__syncwarp();
+				if (lane == 0)
+					umma::mbar_arrive(&drained_bar[stage]);
+				if (++stage == kStages)
+				{
+					stage = 0;
+					phase ^= 1u;
+				}
+			}
+			/* Every MMA of this CTA has run (this warp waited for the last one), and each of them had waited for its copies: the
+			 * slots are free to take the partial sums, token after token. */
+			if (ok)
+			{
+				float *partial = reinterpret_cast<float*>(smem);
+#pragma unroll
+				for (int t = 0; t < TOKENS; t++)
+					partial[t * 128 + threadIdx.x] = acc[t];
+			}
+		}
+
+		__syncthreads();
+		if (abort_flag != 0)
+			umma::drain_after_abort();
+		if (splits > 1)
+			umma::cluster_sync_all(); /* the partial sums of every CTA are written */
+		if (warp < 4 and abort_flag == 0)
+		{
+			const int tokens = min(TOKENS, p.M - m0);
+			const uint32_t partial = umma::smem_u32(smem);
+			for (int i = rank * 128 + threadIdx.x; i < tokens * 32; i += splits * 128)
+			{
+				const int n = i % 32 * 4;
+				float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+				for (int q = 0; q < splits; q++)
+				{
+					float4 v;
+					if (splits > 1)
+						asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+								: "r"(umma::map_to_cta(partial + static_cast<uint32_t>(i) * 16u, static_cast<uint32_t>(q))) : "memory");
+					else
+						v = reinterpret_cast<const float4*>(smem)[i];
+					sum.x += v.x;
+					sum.y += v.y;
+					sum.z += v.z;
+					sum.w += v.w;
+				}
+				if (n0 + n < p.N)
+					finish_four(p, static_cast<long long>(m0 + i / 32) * p.N + n0 + n, sum, min(4, p.N - n0 - n));
+			}
+		}
+		umma::tcgen05_fence_before();
+		__syncthreads();
+		if (splits > 1)
+			umma::cluster_sync_all(); /* nobody leaves while its partial sums may still be read */
+		if (warp == 4)
+		{
+			umma::tcgen05_fence_after();
+			umma::tmem_dealloc(tmem_base, Cfg::kTmemColumns);
+		}
+	}
+
+	int sm_count(const ContextObject &ctx)
+	{
+		int sms = 148;
+		cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx.device);
+		return sms;
+	}
+	bool make_operand_map(CUtensorMap *map, const uint8_t *base, int rows, int k, int boxRows)
+	{
+		const uint64_t dims[2] = { static_cast<uint64_t>(k), static_cast<uint64_t>(rows) };
+		const uint64_t strides[1] = { static_cast<uint64_t>(k) };
+		const uint32_t box[2] = { kScaleBlock, static_cast<uint32_t>(boxRows) };
+		return umma::make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+	}
+
+	/* CTAs per tile: the number that ends first, where a CTA's time is its blocks of K plus about kOverhead blocks of set-up, first
+	 * copy and reduction, and one CTA runs per SM. */
+	int choose_splits(long long tiles, int blocks, int sms)
+	{
+		constexpr int kOverhead = 6;
+		int best = 1;
+		long long best_cost = 0;
+		for (int s = 1; s <= std::min(kMaxSplits, blocks); s++)
+		{
+			const long long waves = (tiles + sms / s - 1) / (sms / s);
+			const long long cost = waves * ((blocks + s - 1) / s + kOverhead);
+			if (s == 1 or cost < best_cost)
+			{
+				best = s;
+				best_cost = cost;
+			}
+		}
+		return best;
+	}
+
+	template<int TOKENS, bool LOADERS>
+	avStatus_t launch_split(ContextObject &ctx, const ScaledGemm &p)
+	{
+		using Cfg = SplitConfig<TOKENS, LOADERS>;
+		auto kernel = kernel_gemm_f8_split<TOKENS, LOADERS>;
+		static PerDeviceOnce configured;
+		if (configured.run(ctx.device, [&]() -> cudaError_t { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes); }) != cudaSuccess)
+		{
+			cudaGetLastError();
+			return AVOCADO_STATUS_EXECUTION_FAILED;
+		}
+		CUtensorMap mapA = { }, mapB = { };
+		if (not LOADERS and (not make_operand_map(&mapA, p.a, p.M, p.K, TOKENS) or not make_operand_map(&mapB, p.b, p.N, p.K, 128)))
+			return AVOCADO_STATUS_INTERNAL_ERROR;
+		const long long token_tiles = (static_cast<long long>(p.M) + TOKENS - 1) / TOKENS;
+		const long long tiles = token_tiles * scale_blocks(p.N);
+		const int splits = choose_splits(tiles, p.blocks, sm_count(ctx));
+		if (tiles * splits > 0x7FFFFFFFll)
+			return AVOCADO_STATUS_NOT_SUPPORTED;
+		cudaLaunchConfig_t config = { };
+		config.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+		config.blockDim = dim3(Cfg::kThreads);
+		config.dynamicSmemBytes = Cfg::kSmemBytes;
+		config.stream = ctx.getStream();
+		cudaLaunchAttribute attributes[2];
+		attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+		attributes[0].val.programmaticStreamSerializationAllowed = chained_launches_enabled() ? 1 : 0;
+		attributes[1].id = cudaLaunchAttributeClusterDimension;
+		attributes[1].val.clusterDim.x = static_cast<unsigned>(splits);
+		attributes[1].val.clusterDim.y = 1;
+		attributes[1].val.clusterDim.z = 1;
+		config.attrs = attributes;
+		config.numAttrs = splits > 1 ? 2 : 1;
+		const cudaError_t launched = cudaLaunchKernelEx(&config, kernel, mapA, mapB, p, static_cast<int>(token_tiles), splits, (p.blocks + splits - 1) / splits,
+				ctx.getDeviceStatus());
+		return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
+	}
+	template<bool LOADERS>
+	avStatus_t launch_split(ContextObject &ctx, const ScaledGemm &p)
+	{
+		if (p.M <= 16)
+			return launch_split<16, LOADERS>(ctx, p);
+		if (p.M <= 32)
+			return launch_split<32, LOADERS>(ctx, p);
+		if (p.M <= 64)
+			return launch_split<64, LOADERS>(ctx, p);
+		return launch_split<128, LOADERS>(ctx, p);
+	}
+
 	avStatus_t launch(ContextObject &ctx, const ScaledGemm &p)
 	{
-		const long long grid = static_cast<long long>((p.M + 63) / 64) * ((p.N + 63) / 64);
-		if (grid > 0x7FFFFFFFll)
-			return AVOCADO_STATUS_NOT_SUPPORTED;
-		const cudaError_t launched = launch_chained(kernel_gemm_f8_simt<T>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx.getStream(), p);
-		return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
+		if (p.K == 0)
+		{
+			const long long wanted = (static_cast<long long>(p.M) * p.N + 255) / 256;
+			const dim3 grid(static_cast<unsigned>(std::min<long long>(wanted, static_cast<long long>(sm_count(ctx)) * 8)));
+			const cudaError_t launched = launch_chained(kernel_scale_c, grid, dim3(256), 0, ctx.getStream(), p);
+			return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
+		}
+		const bool tma = p.K % 16 == 0 and (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0;
+		return tma ? launch_split<false>(ctx, p) : launch_split<true>(ctx, p);
 	}
 }
 
@@ -134,6 +568,9 @@ namespace avocado
 					return AVOCADO_STATUS_BAD_PARAM;
 				if (p.M == 0 or p.N == 0)
 					return AVOCADO_STATUS_SUCCESS;
+				constexpr int kMaxExtent = 1 << 30; /* indices, rounded up to whole tiles, stay in 32 bits */
+				if (p.M > kMaxExtent or p.N > kMaxExtent or p.K > kMaxExtent)
+					return AVOCADO_STATUS_NOT_SUPPORTED;
 				Operand ao, bo, co, as, bs;
 				if (not get_operand(ao, ctx, aMem, a) or not get_operand(bo, ctx, bMem, b) or not get_operand(co, ctx, cMem, c)
 						or not get_operand(as, ctx, aScaleMem, a_scale) or not get_operand(bs, ctx, bScaleMem, b_scale))
@@ -148,15 +585,12 @@ namespace avocado
 				p.alpha = getAlphaValue<float>(alpha);
 				p.beta = getBetaValue<float>(beta);
 				ctx.setDevice();
-				switch (c.dtype)
-				{
-					case AVOCADO_DTYPE_FLOAT16:
-						return launch<half>(ctx, p);
-					case AVOCADO_DTYPE_BFLOAT16:
-						return launch<__nv_bfloat16>(ctx, p);
-					default:
-						return launch<float>(ctx, p);
-				}
+				p.c_type = c.dtype;
+				const int four = 4 * static_cast<int>(dtype_size(c.dtype));
+				p.c_vector = (p.N % 4 == 0 and co.aligned(four)) ? 1 : 0;
+				if (cuda_sm_version(ctx.device) != 100)
+					return AVOCADO_STATUS_NOT_SUPPORTED;
+				return launch(ctx, p);
 			AVOCADO_API_END
 		}
 	} /* namespace backend */

@@ -201,10 +201,10 @@ namespace umma
 		return desc;
 	}
 
-	/* Instruction descriptor (32 bit) of tcgen05.mma kind::f16 / kind::tf32 / kind::i8:
+	/* Instruction descriptor (32 bit) of tcgen05.mma kind::f16 / kind::tf32 / kind::i8 / kind::f8f6f4:
 	 * [5:4] accumulator format (1 = f32, 2 = s32), [9:7] A format, [12:10] B format, [15] A is MN-major,
 	 * [16] B is MN-major, [22:17] N >> 3, [28:24] M >> 4. */
-	constexpr uint32_t kFormatF16 = 0, kFormatBF16 = 1, kFormatTF32 = 2, kFormatS8 = 1;
+	constexpr uint32_t kFormatF16 = 0, kFormatBF16 = 1, kFormatTF32 = 2, kFormatS8 = 1, kFormatE4M3 = 0;
 	constexpr uint32_t kAccumF32 = 1, kAccumS32 = 2;
 
 	__host__ __device__ constexpr uint32_t make_instr_desc(uint32_t accum, uint32_t aFormat, uint32_t bFormat, bool aMnMajor, bool bMnMajor, uint32_t m,
@@ -251,6 +251,7 @@ namespace umma
 	}
 	B200_UMMA_K4(mma_f16_k4, "f16")
 	B200_UMMA_K4(mma_i8_k4, "i8")
+	B200_UMMA_K4(mma_f8_k4, "f8f6f4")
 #undef B200_UMMA_K4
 	/* makes the mbarrier track completion of all MMAs issued so far by this thread (one arrival) */
 	__device__ __forceinline__ void mma_commit(uint64_t *bar)
@@ -366,6 +367,7 @@ namespace umma
 	}
 	B200_UMMA_PAIR_K4(mma_f16_pair_k4, "f16")
 	B200_UMMA_PAIR_K4(mma_i8_pair_k4, "i8")
+	B200_UMMA_PAIR_K4(mma_f8_pair_k4, "f8f6f4")
 #undef B200_UMMA_PAIR_K4
 	/* one arrival on the mbarrier at this offset in every CTA named by the mask, once all MMAs issued so far are done */
 	__device__ __forceinline__ void mma_commit_pair(uint64_t *bar, uint16_t ctaMask)

@@ -152,7 +152,7 @@ DLL_PUBLIC avStatus_t cudaRmsNormQuantize(avContextDescriptor_t context, const a
 /* C = alpha * A * B^T + beta * C for quantised A [M, K] in 1 x 128 blocks and B [N, K] in 128 x 128 blocks:
  *   C[m, n] = alpha * sum over g of aScale[m, g] * bScale[n / 128, g] * (sum over k in block g of A[m, k] * B[n, k]) + beta * C[m, n]
  * aDesc, bDesc: float8_e4m3; scales float32 [M, ceil(K / 128)] and [ceil(N / 128), ceil(K / 128)]; C float16, bfloat16 or
- * float32 [M, N]; alpha and beta float.  aOp must be N and bOp T (AVOCADO_STATUS_NOT_SUPPORTED otherwise).  Sums are float32,
+ * float32 [M, N]; extents up to 2^30; alpha and beta float.  aOp must be N and bOp T (AVOCADO_STATUS_NOT_SUPPORTED otherwise).  Sums are float32,
  * rounded once into C.  C is not read when beta is 0.  Row pitches of 16 bytes (K a multiple of 16, A and B on 16-byte
  * boundaries) are copied by the tensor memory accelerator; other pitches are correct and slower. */
 DLL_PUBLIC avStatus_t cudaGemmBlockScaled(avContextDescriptor_t context, avGemmOperation_t aOp, avGemmOperation_t bOp, const void *alpha,
