@@ -435,6 +435,365 @@ namespace
 		}
 	}
 
+	/*
+	 * Many rows on both sides: pairs of CTAs (cta_group::2) on tiles of 256 x 256.  Each CTA copies its 128 rows of A and its half of
+	 * the rows of B, holds 128 x 256 accumulators in float32 registers (128 per thread of eight warps) and the two newest blocks
+	 * of K in TMEM.
+	 *
+	 * Why 256 x 256: per block of K a CTA pulls 32 KB from L2 for 558 cycles of MMAs (four of N = 256, 139.5 cycles each),
+	 * 59 bytes per cycle; 128 x 128 tiles on single CTAs pull 32 KB for 344 cycles.  The promotion acc += scale * part reads
+	 * 128 x 256 floats of TMEM per block of K and issues 256 packed fused multiply-adds per scheduler, which fits beside the MMAs.
+	 * Why two issuing threads: a block of K costs its issuer two waits, four MMAs and two commits, about 680 cycles, more
+	 * than the MMAs take; even and odd blocks have an issuer (and an accumulator) each.
+	 *
+	 *   full[s]        first CTA only: its producer posts the bytes of both CTAs' copies
+	 *   empty[s]       both CTAs: the commit after a slot's MMAs
+	 *   part_full[b]   both CTAs: the same, for the accumulator
+	 *   part_empty[b]  first CTA only: one arrival per promotion warp of both CTAs
+	 */
+	constexpr int kPairStages = 5;
+	constexpr int kPairSlotBytes = 2 * kBlockBytes; /* 128 rows of A, 128 rows of B */
+	constexpr int kPairControlThreads = 128;        /* producer, two issuers, one warp for TMEM */
+	constexpr int kPairThreads = kPairControlThreads + 256;
+	constexpr int kPairControlRegisters = 40;
+	constexpr int kPairPromoteRegisters = 232;
+	constexpr int kSubBytes = 32 * 128;             /* a warp's 32 rows, 128 bytes of C each */
+	constexpr int kPairSmemBytes = kPairStages * kPairSlotBytes + 8 * 2 * kSubBytes + 1024;
+	static_assert(kPairSmemBytes <= 232448 - 512, "shared memory of an SM");
+	static_assert(kPairControlThreads * kPairControlRegisters + 256 * kPairPromoteRegisters <= kPairThreads * 168, "registers of the launch");
+	constexpr int kBandRows = 8; /* tiles are walked in bands of this many tile rows, column by column, so that neighbours in time share operands in L2 */
+
+	struct PairTile
+	{
+			int m, n;
+	};
+	__device__ __forceinline__ PairTile pair_tile(int tile, int mBlocks, int nBlocks)
+	{
+		const int band = tile / (kBandRows * nBlocks);
+		const int rows = min(kBandRows, mBlocks - band * kBandRows);
+		const int r = tile - band * kBandRows * nBlocks;
+		PairTile t;
+		t.m = band * kBandRows + r % rows;
+		t.n = r / rows;
+		return t;
+	}
+	__device__ __forceinline__ unsigned long long pack2(uint32_t x, uint32_t y)
+	{
+		unsigned long long v;
+		asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(x), "r"(y));
+		return v;
+	}
+	__device__ __forceinline__ float2 unpack2(unsigned long long v)
+	{
+		float2 r;
+		asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+		return r;
+	}
+	__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c)
+	{
+		unsigned long long r;
+		asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+		return r;
+	}
+
+	/* One 32-row sub-tile of C (64 16-bit or 32 float32 columns) from registers: staged in the swizzled order of the store's tensor
+	 * map, then written by one bulk copy, or row by row where C's pitch or address rules the copy out. */
+	template<bool WIDE>
+	__device__ __forceinline__ void store_sub_tile(const ScaledGemm &p, const CUtensorMap *mapC, uint8_t *buffer, const unsigned long long *acc, int row0, int column0,
+			int lane, bool bulk)
+	{
+		constexpr int kColumns = WIDE ? 32 : 64;
+		constexpr int kPerPiece = WIDE ? 4 : 8; /* elements of 16 bytes */
+		if (row0 >= p.M or column0 >= p.N)
+			return;
+		if (bulk)
+		{
+			if (lane == 0)
+				umma::tma_store_wait_read<1>(); /* the copy before last has read this buffer */
+			__syncwarp();
+		}
+		const long long row = row0 + lane;
+		const bool add = p.beta != 0.0f and row < p.M;
+#pragma unroll
+		for (int j = 0; j < kColumns / kPerPiece; j++)
+		{
+			float x[kPerPiece];
+#pragma unroll
+			for (int i = 0; i < kPerPiece; i += 2)
+			{
+				const float2 v = unpack2(acc[(j * kPerPiece + i) / 2]);
+				x[i] = p.alpha * v.x;
+				x[i + 1] = p.alpha * v.y;
+			}
+			if (add)
+			{
+#pragma unroll
+				for (int i = 0; i < kPerPiece; i++)
+					if (column0 + j * kPerPiece + i < p.N)
+						x[i] = fmaf(p.beta, load_c(p, row * p.N + column0 + j * kPerPiece + i), x[i]);
+			}
+			uint4 piece;
+			if constexpr (WIDE)
+				piece = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+			else
+				piece = make_uint4(pack_two(p.c_type, x[0], x[1]), pack_two(p.c_type, x[2], x[3]), pack_two(p.c_type, x[4], x[5]), pack_two(p.c_type, x[6], x[7]));
+			*reinterpret_cast<uint4*>(buffer + lane * 128 + ((j ^ (lane & 7)) << 4)) = piece;
+		}
+		if (bulk)
+		{
+			umma::fence_proxy_async_smem();
+			__syncwarp();
+			if (lane == 0)
+			{
+				umma::tma_store_2d(mapC, buffer, column0, row0);
+				umma::tma_store_commit();
+			}
+		}
+		else
+		{
+			__syncwarp();
+			for (int r = 0; r < min(32, p.M - row0); r++)
+#pragma unroll
+				for (int i = 0; i < kColumns / 32; i++)
+				{
+					const int column = i * 32 + lane;
+					const uint8_t *at = buffer + r * 128 + (((column / kPerPiece) ^ (r & 7)) << 4);
+					const long long to = static_cast<long long>(row0 + r) * p.N + column0 + column;
+					if (column0 + column < p.N)
+					{
+						if constexpr (WIDE)
+							reinterpret_cast<float*>(p.c)[to] = reinterpret_cast<const float*>(at)[column % kPerPiece];
+						else
+							reinterpret_cast<uint16_t*>(p.c)[to] = reinterpret_cast<const uint16_t*>(at)[column % kPerPiece];
+					}
+				}
+			__syncwarp();
+		}
+	}
+
+	__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) kernel_gemm_f8_pair(const __grid_constant__ CUtensorMap mapA,
+			const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapC, ScaledGemm p, int mBlocks, int nBlocks, int numTiles, int bulkStore,
+			int *deviceStatus)
+	{
+		extern __shared__ uint8_t smem_raw[];
+		uint8_t *smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+
+		__shared__ __align__(8) uint64_t full_bar[kPairStages];
+		__shared__ __align__(8) uint64_t empty_bar[kPairStages];
+		__shared__ __align__(8) uint64_t part_full_bar[2];
+		__shared__ __align__(8) uint64_t part_empty_bar[2];
+		__shared__ uint32_t tmem_base_slot;
+		__shared__ int abort_flag;
+
+		const int warp = threadIdx.x / 32;
+		const int lane = threadIdx.x % 32;
+		const int rank = static_cast<int>(umma::cluster_cta_rank());
+		const int pair = blockIdx.x / 2;
+		const int pairs = gridDim.x / 2;
+
+		if (threadIdx.x == 0)
+		{
+			abort_flag = 0;
+			for (int s = 0; s < kPairStages; s++)
+			{
+				umma::mbar_init(&full_bar[s], 1);
+				umma::mbar_init(&empty_bar[s], 1);
+			}
+			for (int b = 0; b < 2; b++)
+			{
+				umma::mbar_init(&part_full_bar[b], 1);
+				umma::mbar_init(&part_empty_bar[b], 2 * 8);
+			}
+			umma::mbar_fence_init();
+			umma::prefetch_tensormap(&mapA);
+			umma::prefetch_tensormap(&mapB);
+			if (bulkStore)
+				umma::prefetch_tensormap(&mapC);
+		}
+		if (warp == 3)
+		{
+			umma::tmem_alloc_pair(&tmem_base_slot, 512);
+			umma::tmem_relinquish_pair();
+		}
+		umma::tcgen05_fence_before();
+		__syncthreads();
+		umma::cluster_sync_all(); /* both CTAs' barriers exist before anything arrives on them */
+		umma::tcgen05_fence_after();
+		const uint32_t tmem_base = tmem_base_slot;
+		volatile int *abort_ptr = &abort_flag;
+		chain_release();
+		chain_wait();
+
+		if (warp < kPairControlThreads / 32)
+		{
+			asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairControlRegisters));
+		}
+		if (warp == 0)
+		{
+			if (lane == 0)
+			{
+				int stage = 0;
+				uint32_t phase = 0;
+				bool ok = true;
+				for (int tile = pair; tile < numTiles and ok; tile += pairs)
+				{
+					const PairTile t = pair_tile(tile, mBlocks, nBlocks);
+					const int m0 = t.m * 256 + rank * 128, n0 = t.n * 256 + rank * 128;
+					for (int kb = 0; kb < p.blocks; kb++)
+					{
+						if (not umma::mbar_wait(&empty_bar[stage], phase ^ 1u, abort_ptr))
+						{
+							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorStageWait);
+							ok = false;
+							break;
+						}
+						const uint32_t bar = umma::map_to_cta(umma::smem_u32(&full_bar[stage]), 0);
+						if (rank == 0)
+							umma::mbar_arrive_expect_tx(&full_bar[stage], 2 * kPairSlotBytes);
+						uint8_t *slot = smem + stage * kPairSlotBytes;
+						umma::tma_load_2d_pair(slot, &mapA, bar, kb * kScaleBlock, m0);
+						umma::tma_load_2d_pair(slot + kBlockBytes, &mapB, bar, kb * kScaleBlock, n0);
+						if (++stage == kPairStages)
+						{
+							stage = 0;
+							phase ^= 1u;
+						}
+					}
+				}
+			}
+		}
+		else if (warp == 1 or warp == 2)
+		{
+			if (lane == 0 and rank == 0)
+			{
+				/* issuer b takes the blocks b, b + 2, ... of the whole sequence of tiles, whose slots are two apart */
+				constexpr uint32_t idesc = umma::make_instr_desc(umma::kAccumF32, umma::kFormatE4M3, umma::kFormatE4M3, false, false, 256, 256);
+				const uint64_t desc0 = umma::make_smem_desc(umma::smem_u32(smem), 16, 1024, umma::kSwizzle128B);
+				const int b = warp - 1;
+				const uint32_t part = tmem_base + static_cast<uint32_t>(b * 256);
+				const int tiles = (numTiles - pair + pairs - 1) / pairs;
+				const long long total = static_cast<long long>(tiles) * p.blocks;
+				int stage = b;
+				uint32_t phase = 0, part_phase = 0;
+				for (long long i = b; i < total; i += 2)
+				{
+					if (not umma::mbar_wait(&part_empty_bar[b], part_phase ^ 1u, abort_ptr))
+					{
+						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorMmaWait);
+						break;
+					}
+					if (not umma::mbar_wait(&full_bar[stage], phase, abort_ptr))
+					{
+						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorTmaWait);
+						break;
+					}
+					umma::tcgen05_fence_after();
+					const uint64_t desc = desc0 + static_cast<uint64_t>(stage * (kPairSlotBytes / 16));
+					umma::mma_f8_pair_k4(part, desc, desc + kBlockBytes / 16, idesc, false);
+					umma::mma_commit_pair(&empty_bar[stage], 3);
+					umma::mma_commit_pair(&part_full_bar[b], 3); /* last: who has seen it need not expect another arrival */
+					part_phase ^= 1u;
+					stage += 2;
+					if (stage >= kPairStages)
+					{
+						stage -= kPairStages;
+						phase ^= 1u;
+					}
+				}
+			}
+		}
+		else if (warp >= kPairControlThreads / 32)
+		{
+			asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairPromoteRegisters));
+			const int quarter = warp % 4;
+			const int half = (warp - kPairControlThreads / 32) / 4;
+			const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * 128);
+			uint8_t *buffers = smem + kPairStages * kPairSlotBytes + (warp - kPairControlThreads / 32) * 2 * kSubBytes;
+			uint32_t b = 0, phase = 0;
+			bool ok = true;
+			for (int tile = pair; tile < numTiles and ok; tile += pairs)
+			{
+				const PairTile t = pair_tile(tile, mBlocks, nBlocks);
+				const int row0 = t.m * 256 + rank * 128 + quarter * 32;
+				const int column0 = t.n * 256 + half * 128;
+				/* rows and columns past the end have products of zeros: any scale will do, the last one's is there */
+				const float *a_scale = p.a_scale + static_cast<long long>(min(row0 + lane, p.M - 1)) * p.blocks;
+				const float *b_scale = p.b_scale + static_cast<long long>(min(column0, p.N - 1) / kScaleBlock) * p.blocks;
+				unsigned long long acc[64];
+#pragma unroll
+				for (int i = 0; i < 64; i++)
+					acc[i] = 0;
+				float next_a = a_scale[0], next_b = b_scale[0];
+				for (int kb = 0; kb < p.blocks; kb++)
+				{
+					const uint32_t s = __float_as_uint(next_a * next_b);
+					const unsigned long long scale = pack2(s, s);
+					const int ahead = min(kb + 1, p.blocks - 1);
+					next_a = a_scale[ahead];
+					next_b = b_scale[ahead];
+					ok = __all_sync(0xFFFFFFFFu, umma::mbar_wait(&part_full_bar[b], phase, abort_ptr));
+					if (not ok)
+					{
+						if (lane == 0)
+							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
+						break;
+					}
+					umma::tcgen05_fence_after();
+					const uint32_t from = lanes + b * 256u;
+					uint32_t r[2][32];
+					umma::tmem_load_32x32(from, r[0]);
+#pragma unroll
+					for (int chunk = 0; chunk < 4; chunk++)
+					{
+						umma::tmem_load_wait();
+						if (chunk < 3)
+							umma::tmem_load_32x32(from + static_cast<uint32_t>((chunk + 1) * 32), r[(chunk + 1) & 1]);
+						else
+						{
+							umma::tcgen05_fence_before();
+							__syncwarp();
+							if (lane == 0)
+								umma::mbar_arrive_cluster(umma::map_to_cta(umma::smem_u32(&part_empty_bar[b]), 0));
+						}
+#pragma unroll
+						for (int i = 0; i < 16; i++)
+							acc[chunk * 16 + i] = fma2(pack2(r[chunk & 1][2 * i], r[chunk & 1][2 * i + 1]), scale, acc[chunk * 16 + i]);
+					}
+					if ((b ^= 1u) == 0)
+						phase ^= 1u;
+				}
+				if (not ok)
+					break;
+				if (p.c_type == AVOCADO_DTYPE_FLOAT32)
+				{
+#pragma unroll
+					for (int sub = 0; sub < 4; sub++)
+						store_sub_tile<true>(p, &mapC, buffers + (sub & 1) * kSubBytes, acc + sub * 16, row0, column0 + sub * 32, lane, bulkStore != 0);
+				}
+				else
+				{
+#pragma unroll
+					for (int sub = 0; sub < 2; sub++)
+						store_sub_tile<false>(p, &mapC, buffers + sub * kSubBytes, acc + sub * 32, row0, column0 + sub * 64, lane, bulkStore != 0);
+				}
+			}
+			if (lane == 0)
+				umma::tma_store_wait_all<0>();
+		}
+
+		/* neither CTA may leave (or free TMEM) while the other can still touch its shared memory, barriers or TMEM */
+		__syncthreads();
+		if (abort_flag != 0)
+			umma::drain_after_abort();
+		umma::tcgen05_fence_before();
+		umma::cluster_sync_all();
+		if (warp == 3)
+		{
+			umma::tcgen05_fence_after();
+			umma::tmem_dealloc_pair(tmem_base, 512);
+		}
+	}
+
 	int sm_count(const ContextObject &ctx)
 	{
 		int sms = 148;
@@ -518,6 +877,40 @@ namespace
 		return launch_split<128, LOADERS>(ctx, p);
 	}
 
+	avStatus_t launch_pair(ContextObject &ctx, const ScaledGemm &p)
+	{
+		auto kernel = kernel_gemm_f8_pair;
+		static PerDeviceOnce configured;
+		if (configured.run(ctx.device, [&]() -> cudaError_t { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes); }) != cudaSuccess)
+		{
+			cudaGetLastError();
+			return AVOCADO_STATUS_EXECUTION_FAILED;
+		}
+		CUtensorMap mapA, mapB, mapC = { };
+		if (not make_operand_map(&mapA, p.a, p.M, p.K, 128) or not make_operand_map(&mapB, p.b, p.N, p.K, 128))
+			return AVOCADO_STATUS_INTERNAL_ERROR;
+		const int size = p.c_type == AVOCADO_DTYPE_FLOAT32 ? 4 : 2;
+		const bool bulk = static_cast<long long>(p.N) * size % 16 == 0 and reinterpret_cast<uintptr_t>(p.c) % 16 == 0;
+		if (bulk)
+		{
+			const CUtensorMapDataType type = p.c_type == AVOCADO_DTYPE_FLOAT32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 :
+					p.c_type == AVOCADO_DTYPE_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+			const uint64_t dims[2] = { static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M) };
+			const uint64_t strides[1] = { static_cast<uint64_t>(p.N) * size };
+			const uint32_t box[2] = { static_cast<uint32_t>(128 / size), 32 };
+			if (not umma::make_tensor_map(&mapC, type, 2, p.c, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+				return AVOCADO_STATUS_INTERNAL_ERROR;
+		}
+		const int m_blocks = (p.M + 255) / 256, n_blocks = (p.N + 255) / 256;
+		const long long tiles = static_cast<long long>(m_blocks) * n_blocks;
+		if (tiles > 0x3FFFFFFFll)
+			return AVOCADO_STATUS_NOT_SUPPORTED;
+		const int pairs = static_cast<int>(std::min<long long>(tiles, sm_count(ctx) / 2));
+		const cudaError_t launched = launch_chained(kernel, dim3(2 * pairs), dim3(kPairThreads), kPairSmemBytes, ctx.getStream(), mapA, mapB, mapC, p, m_blocks,
+				n_blocks, static_cast<int>(tiles), bulk ? 1 : 0, ctx.getDeviceStatus());
+		return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
+	}
+
 	avStatus_t launch(ContextObject &ctx, const ScaledGemm &p)
 	{
 		if (p.K == 0)
@@ -528,6 +921,8 @@ namespace
 			return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
 		}
 		const bool tma = p.K % 16 == 0 and (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0;
+		if (tma and static_cast<long long>((p.M + 255) / 256) * ((p.N + 255) / 256) >= 32)
+			return launch_pair(ctx, p);
 		return tma ? launch_split<false>(ctx, p) : launch_split<true>(ctx, p);
 	}
 }

@@ -58,6 +58,34 @@ def test_odd_row_pitches(ctx, dtype, shape):
     p.check()
 
 
+# enough tiles of 256 x 256 for the CTA-pair kernel: ragged rows and columns, C pitches that no bulk copy takes, one block of K
+PAIR_SHAPES = [(2049, 1025, 272), (1500, 1501, 144), (8200, 130, 256), (257, 8004, 400), (5000, 520, 16), (2300, 2302, 1024)]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("shape", PAIR_SHAPES)
+@pytest.mark.parametrize("alpha,beta", [(1.0, 0.0), (-0.6, 0.7)])
+def test_many_rows_on_both_sides(ctx, dtype, shape, alpha, beta):
+    p = Problem(ctx, *shape, dtype, c_offset=4 if shape[1] == 8004 else 0)
+    p.run(alpha, beta)
+    p.check(alpha, beta)
+
+
+@pytest.mark.parametrize("k", [128, 256, 384, 1408])
+def test_exact_on_large_tiles(ctx, k):
+    """integers and powers of two through the CTA-pair kernel: even and odd numbers of blocks per tile"""
+    m, n = 3333, 1100
+    p = Problem(ctx, m, n, k, "float32")
+    r = np.random.default_rng(94)
+    p.a.upload(r.integers(-8, 9, (m, k)))
+    p.b.upload(r.integers(-8, 9, (n, k)))
+    p.sa.upload(np.exp2(r.integers(-2, 2, (m, bs.blocks(k)))))
+    p.sb.upload(np.exp2(r.integers(-2, 2, (bs.blocks(n), bs.blocks(k)))))
+    for _ in range(2):
+        p.run()
+        assert np.array_equal(p.c.download(), p.expected()[0])
+
+
 @pytest.mark.parametrize("a_offset,b_offset,c_offset", [(1, 0, 0), (0, 2, 0), (4, 4, 0), (8, 0, 2), (0, 8, 4), (0, 0, 2), (0, 0, 8), (16, 32, 16)])
 @pytest.mark.parametrize("shape", [(3, 264, 256), (140, 300, 272), (600, 512, 256)])
 def test_unaligned_views(ctx, a_offset, b_offset, c_offset, shape):
