@@ -361,7 +361,7 @@ namespace
 					{
 						uint32_t r[16];
 						umma::tmem_load_32x16(lanes + static_cast<uint32_t>((stage * kPerStage + j) * TOKENS + t0), r);
-						umma::tmem_load_wait();
+						umma::tmem_load_wait(r);
 #pragma unroll
 						for (int t = 0; t < 16; t += 4)
 						{
@@ -448,18 +448,19 @@ namespace
 	 *
 	 *   full[s]        first CTA only: its producer posts the bytes of both CTAs' copies
 	 *   empty[s]       both CTAs: the commit after a slot's MMAs
-	 *   part_full[b]   both CTAs: the same, for the accumulator
+	 *   part_full[b]   both CTAs: the same, for the accumulator, and one arrival of the CTA's own warp that brings the scales
 	 *   part_empty[b]  first CTA only: one arrival per promotion warp of both CTAs
 	 */
 	constexpr int kPairStages = 5;
 	constexpr int kPairSlotBytes = 2 * kBlockBytes; /* 128 rows of A, 128 rows of B */
-	constexpr int kPairControlThreads = 128;        /* producer, two issuers, one warp for TMEM */
+	constexpr int kPairControlThreads = 128;        /* producer, two issuers, one warp for the scales (and TMEM) */
 	constexpr int kPairThreads = kPairControlThreads + 256;
 	constexpr int kPairControlRegisters = 40;
 	constexpr int kPairPromoteRegisters = 232;
+	constexpr int kScaleSlots = 3, kScaleAhead = 3; /* blocks of K whose scales are in shared memory, and in flight to it */
 	constexpr int kSubBytes = 32 * 128;             /* a warp's 32 rows, 128 bytes of C each */
 	constexpr int kPairSmemBytes = kPairStages * kPairSlotBytes + 8 * 2 * kSubBytes + 1024;
-	static_assert(kPairSmemBytes <= 232448 - 512, "shared memory of an SM");
+	static_assert(kPairSmemBytes <= 232448 - 256 - kScaleSlots * 130 * 4, "shared memory of an SM");
 	static_assert(kPairControlThreads * kPairControlRegisters + 256 * kPairPromoteRegisters <= kPairThreads * 168, "registers of the launch");
 	constexpr int kBandRows = 8; /* tiles are walked in bands of this many tile rows, column by column, so that neighbours in time share operands in L2 */
 
@@ -477,29 +478,10 @@ namespace
 		t.n = r / rows;
 		return t;
 	}
-	__device__ __forceinline__ unsigned long long pack2(uint32_t x, uint32_t y)
-	{
-		unsigned long long v;
-		asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(x), "r"(y));
-		return v;
-	}
-	__device__ __forceinline__ float2 unpack2(unsigned long long v)
-	{
-		float2 r;
-		asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-		return r;
-	}
-	__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c)
-	{
-		unsigned long long r;
-		asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-		return r;
-	}
-
 	/* One 32-row sub-tile of C (64 16-bit or 32 float32 columns) from registers: staged in the swizzled order of the store's tensor
 	 * map, then written by one bulk copy, or row by row where C's pitch or address rules the copy out. */
 	template<bool WIDE>
-	__device__ __forceinline__ void store_sub_tile(const ScaledGemm &p, const CUtensorMap *mapC, uint8_t *buffer, const unsigned long long *acc, int row0, int column0,
+	__device__ __forceinline__ void store_sub_tile(const ScaledGemm &p, const CUtensorMap *mapC, uint8_t *buffer, const float *acc, int row0, int column0,
 			int lane, bool bulk)
 	{
 		constexpr int kColumns = WIDE ? 32 : 64;
@@ -521,9 +503,8 @@ namespace
 #pragma unroll
 			for (int i = 0; i < kPerPiece; i += 2)
 			{
-				const float2 v = unpack2(acc[(j * kPerPiece + i) / 2]);
-				x[i] = p.alpha * v.x;
-				x[i + 1] = p.alpha * v.y;
+				x[i] = p.alpha * acc[j * kPerPiece + i];
+				x[i + 1] = p.alpha * acc[j * kPerPiece + i + 1];
 			}
 			if (add)
 			{
@@ -580,10 +561,12 @@ namespace
 
 		__shared__ __align__(8) uint64_t full_bar[kPairStages];
 		__shared__ __align__(8) uint64_t empty_bar[kPairStages];
-		__shared__ __align__(8) uint64_t part_full_bar[2];
-		__shared__ __align__(8) uint64_t part_empty_bar[2];
+		__shared__ __align__(8) uint64_t part_full_bar[4];
+		__shared__ __align__(8) uint64_t part_empty_bar[4];
 		__shared__ uint32_t tmem_base_slot;
 		__shared__ int abort_flag;
+		__shared__ __align__(16) float a_scale_s[kScaleSlots][128];
+		__shared__ __align__(16) float b_scale_s[kScaleSlots][2];
 
 		const int warp = threadIdx.x / 32;
 		const int lane = threadIdx.x % 32;
@@ -599,10 +582,10 @@ namespace
 				umma::mbar_init(&full_bar[s], 1);
 				umma::mbar_init(&empty_bar[s], 1);
 			}
-			for (int b = 0; b < 2; b++)
+			for (int b = 0; b < 4; b++)
 			{
-				umma::mbar_init(&part_full_bar[b], 1);
-				umma::mbar_init(&part_empty_bar[b], 2 * 8);
+				umma::mbar_init(&part_full_bar[b], 2);
+				umma::mbar_init(&part_empty_bar[b], 2 * 4);
 			}
 			umma::mbar_fence_init();
 			umma::prefetch_tensormap(&mapA);
@@ -667,31 +650,38 @@ namespace
 			if (lane == 0 and rank == 0)
 			{
 				/* issuer b takes the blocks b, b + 2, ... of the whole sequence of tiles, whose slots are two apart */
-				constexpr uint32_t idesc = umma::make_instr_desc(umma::kAccumF32, umma::kFormatE4M3, umma::kFormatE4M3, false, false, 256, 256);
+				constexpr uint32_t idesc = umma::make_instr_desc(umma::kAccumF32, umma::kFormatE4M3, umma::kFormatE4M3, false, false, 256, 128);
 				const uint64_t desc0 = umma::make_smem_desc(umma::smem_u32(smem), 16, 1024, umma::kSwizzle128B);
 				const int b = warp - 1;
-				const uint32_t part = tmem_base + static_cast<uint32_t>(b * 256);
 				const int tiles = (numTiles - pair + pairs - 1) / pairs;
 				const long long total = static_cast<long long>(tiles) * p.blocks;
 				int stage = b;
 				uint32_t phase = 0, part_phase = 0;
-				for (long long i = b; i < total; i += 2)
+				bool ok = true;
+				for (long long i = b; i < total and ok; i += 2)
 				{
-					if (not umma::mbar_wait(&part_empty_bar[b], part_phase ^ 1u, abort_ptr))
-					{
-						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorMmaWait);
-						break;
-					}
 					if (not umma::mbar_wait(&full_bar[stage], phase, abort_ptr))
 					{
 						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorTmaWait);
 						break;
 					}
-					umma::tcgen05_fence_after();
 					const uint64_t desc = desc0 + static_cast<uint64_t>(stage * (kPairSlotBytes / 16));
-					umma::mma_f8_pair_k4(part, desc, desc + kBlockBytes / 16, idesc, false);
-					umma::mma_commit_pair(&empty_bar[stage], 3);
-					umma::mma_commit_pair(&part_full_bar[b], 3); /* last: who has seen it need not expect another arrival */
+#pragma unroll
+					for (int h = 0; h < 2; h++)
+					{
+						if (not umma::mbar_wait(&part_empty_bar[2 * b + h], part_phase ^ 1u, abort_ptr))
+						{
+							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorMmaWait);
+							ok = false;
+							break;
+						}
+						umma::tcgen05_fence_after();
+						/* rows h * 64 .. h * 64 + 63 of each CTA's half of B */
+						umma::mma_f8_pair_k4(tmem_base + static_cast<uint32_t>((2 * b + h) * 128), desc, desc + (kBlockBytes + h * 64 * 128) / 16, idesc, false);
+						if (h == 1)
+							umma::mma_commit_pair(&empty_bar[stage], 3);
+						umma::mma_commit_pair(&part_full_bar[2 * b + h], 3); /* the last one: who has seen it need not expect another arrival */
+					}
 					part_phase ^= 1u;
 					stage += 2;
 					if (stage >= kPairStages)
@@ -702,6 +692,67 @@ namespace
 				}
 			}
 		}
+		else if (warp == 3)
+		{
+			/* Scales of this CTA's 128 rows and of the two column halves, four rows per lane, loaded kScaleAhead blocks before they are
+			 * needed.  Slot i % 3 is free for block i once the accumulators of block i - 1 are full: their MMAs waited until every warp had
+			 * taken block i - 3, and with it that block's scales. */
+			float ahead_a[kScaleAhead][4], ahead_b[kScaleAhead];
+			const int tiles = (numTiles - pair + pairs - 1) / pairs;
+			const long long total = static_cast<long long>(tiles) * p.blocks;
+			int load_tile = pair, load_kb = 0;
+			auto fetch = [&](float (&va)[4], float &vb)
+			{
+				/* rows and columns past the end have products of zeros: any scale will do, the last one's is there */
+				const PairTile t = pair_tile(min(load_tile, numTiles - 1), mBlocks, nBlocks);
+				const int row0 = t.m * 256 + rank * 128 + lane;
+#pragma unroll
+				for (int j = 0; j < 4; j++)
+					va[j] = p.a_scale[static_cast<long long>(min(row0 + j * 32, p.M - 1)) * p.blocks + load_kb];
+				vb = p.b_scale[static_cast<long long>(min(t.n * 2 + (lane & 1), (p.N - 1) / kScaleBlock)) * p.blocks + load_kb];
+				if (++load_kb == p.blocks)
+				{
+					load_kb = 0;
+					load_tile += pairs;
+				}
+			};
+#pragma unroll
+			for (int d = 0; d < kScaleAhead; d++)
+				fetch(ahead_a[d], ahead_b[d]);
+			bool ok = true;
+			for (long long i0 = 0; i0 < total and ok; i0 += kScaleAhead)
+			{
+#pragma unroll
+				for (int d = 0; d < kScaleAhead; d++)
+				{
+					const long long i = i0 + d;
+					if (i >= total)
+						break;
+					static_assert(kScaleSlots == kScaleAhead, "slot of block i0 + d");
+					if (i >= 1)
+					{
+						const uint32_t phase = static_cast<uint32_t>((i - 1) >> 1) & 1u;
+						uint64_t *bars = &part_full_bar[((i - 1) & 1) * 2];
+						ok = __all_sync(0xFFFFFFFFu, umma::mbar_wait(bars, phase, abort_ptr) and umma::mbar_wait(bars + 1, phase, abort_ptr));
+						if (not ok)
+						{
+							if (lane == 0)
+								umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
+							break;
+						}
+					}
+#pragma unroll
+					for (int j = 0; j < 4; j++)
+						a_scale_s[d][j * 32 + lane] = ahead_a[d][j];
+					if (lane < 2)
+						b_scale_s[d][lane] = ahead_b[d];
+					__syncwarp();
+					if (lane < 2)
+						umma::mbar_arrive(&part_full_bar[(i & 1) * 2 + lane]);
+					fetch(ahead_a[d], ahead_b[d]);
+				}
+			}
+		}
 		else if (warp >= kPairControlThreads / 32)
 		{
 			asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairPromoteRegisters));
@@ -709,29 +760,22 @@ namespace
 			const int half = (warp - kPairControlThreads / 32) / 4;
 			const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * 128);
 			uint8_t *buffers = smem + kPairStages * kPairSlotBytes + (warp - kPairControlThreads / 32) * 2 * kSubBytes;
-			uint32_t b = 0, phase = 0;
+			uint32_t b = 0, phase = 0, slot = 0;
 			bool ok = true;
 			for (int tile = pair; tile < numTiles and ok; tile += pairs)
 			{
 				const PairTile t = pair_tile(tile, mBlocks, nBlocks);
 				const int row0 = t.m * 256 + rank * 128 + quarter * 32;
-				const int column0 = t.n * 256 + half * 128;
-				/* rows and columns past the end have products of zeros: any scale will do, the last one's is there */
-				const float *a_scale = p.a_scale + static_cast<long long>(min(row0 + lane, p.M - 1)) * p.blocks;
-				const float *b_scale = p.b_scale + static_cast<long long>(min(column0, p.N - 1) / kScaleBlock) * p.blocks;
-				unsigned long long acc[64];
+				/* columns 0..63 of this warp's accumulator come from the first CTA's rows of B, 64..127 from the second's */
+				const int column0 = t.n * 256 + half * 64;
+				float acc[128];
 #pragma unroll
-				for (int i = 0; i < 64; i++)
-					acc[i] = 0;
-				float next_a = a_scale[0], next_b = b_scale[0];
+				for (int i = 0; i < 128; i++)
+					acc[i] = 0.0f;
 				for (int kb = 0; kb < p.blocks; kb++)
 				{
-					const uint32_t s = __float_as_uint(next_a * next_b);
-					const unsigned long long scale = pack2(s, s);
-					const int ahead = min(kb + 1, p.blocks - 1);
-					next_a = a_scale[ahead];
-					next_b = b_scale[ahead];
-					ok = __all_sync(0xFFFFFFFFu, umma::mbar_wait(&part_full_bar[b], phase, abort_ptr));
+					uint64_t *bar = &part_full_bar[2 * b + half];
+					ok = __all_sync(0xFFFFFFFFu, umma::mbar_wait(bar, phase, abort_ptr));
 					if (not ok)
 					{
 						if (lane == 0)
@@ -740,24 +784,27 @@ namespace
 					}
 					umma::tcgen05_fence_after();
 					const uint32_t from = lanes + b * 256u;
-					uint32_t r[2][32];
-					umma::tmem_load_32x32(from, r[0]);
+					uint32_t r[2][16];
+					umma::tmem_load_32x16(from, r[0]);
+					const float a_scale = a_scale_s[slot][quarter * 32 + lane];
+					const float scale[2] = { a_scale * b_scale_s[slot][0], a_scale * b_scale_s[slot][1] };
+					slot = slot == kScaleSlots - 1 ? 0 : slot + 1;
 #pragma unroll
-					for (int chunk = 0; chunk < 4; chunk++)
+					for (int chunk = 0; chunk < 8; chunk++)
 					{
-						umma::tmem_load_wait();
-						if (chunk < 3)
-							umma::tmem_load_32x32(from + static_cast<uint32_t>((chunk + 1) * 32), r[(chunk + 1) & 1]);
+						umma::tmem_load_wait(r[chunk & 1]);
+						if (chunk < 7)
+							umma::tmem_load_32x16(from + static_cast<uint32_t>((chunk + 1) * 16), r[(chunk + 1) & 1]);
 						else
 						{
 							umma::tcgen05_fence_before();
 							__syncwarp();
 							if (lane == 0)
-								umma::mbar_arrive_cluster(umma::map_to_cta(umma::smem_u32(&part_empty_bar[b]), 0));
+								umma::mbar_arrive_cluster_relaxed(umma::map_to_cta(umma::smem_u32(&part_empty_bar[2 * b + half]), 0));
 						}
 #pragma unroll
 						for (int i = 0; i < 16; i++)
-							acc[chunk * 16 + i] = fma2(pack2(r[chunk & 1][2 * i], r[chunk & 1][2 * i + 1]), scale, acc[chunk * 16 + i]);
+							acc[chunk * 16 + i] = fmaf(__uint_as_float(r[chunk & 1][i]), scale[chunk / 4], acc[chunk * 16 + i]);
 					}
 					if ((b ^= 1u) == 0)
 						phase ^= 1u;
@@ -768,13 +815,13 @@ namespace
 				{
 #pragma unroll
 					for (int sub = 0; sub < 4; sub++)
-						store_sub_tile<true>(p, &mapC, buffers + (sub & 1) * kSubBytes, acc + sub * 16, row0, column0 + sub * 32, lane, bulkStore != 0);
+						store_sub_tile<true>(p, &mapC, buffers + (sub & 1) * kSubBytes, acc + sub * 32, row0, column0 + (sub / 2) * 128 + (sub % 2) * 32, lane, bulkStore != 0);
 				}
 				else
 				{
 #pragma unroll
 					for (int sub = 0; sub < 2; sub++)
-						store_sub_tile<false>(p, &mapC, buffers + sub * kSubBytes, acc + sub * 32, row0, column0 + sub * 64, lane, bulkStore != 0);
+						store_sub_tile<false>(p, &mapC, buffers + sub * kSubBytes, acc + sub * 64, row0, column0 + sub * 128, lane, bulkStore != 0);
 				}
 			}
 			if (lane == 0)
