@@ -480,12 +480,12 @@ namespace
 	}
 	/* One 32-row sub-tile of C (64 16-bit or 32 float32 columns) from registers: staged in the swizzled order of the store's tensor
 	 * map, then written by one bulk copy, or row by row where C's pitch or address rules the copy out. */
-	template<bool WIDE>
-	__device__ __forceinline__ void store_sub_tile(const ScaledGemm &p, const CUtensorMap *mapC, uint8_t *buffer, const float *acc, int row0, int column0,
-			int lane, bool bulk)
+	template<typename T, bool ADD>
+	__device__ __forceinline__ void store_sub_tile(const ScaledGemm &p, const CUtensorMap *mapC, uint8_t *buffer, const float *acc, int row0, int column0, int lane,
+			bool bulk)
 	{
-		constexpr int kColumns = WIDE ? 32 : 64;
-		constexpr int kPerPiece = WIDE ? 4 : 8; /* elements of 16 bytes */
+		constexpr int kColumns = 128 / static_cast<int>(sizeof(T));
+		constexpr int kPerPiece = 16 / static_cast<int>(sizeof(T));
 		if (row0 >= p.M or column0 >= p.N)
 			return;
 		if (bulk)
@@ -494,31 +494,37 @@ namespace
 				umma::tma_store_wait_read<1>(); /* the copy before last has read this buffer */
 			__syncwarp();
 		}
-		const long long row = row0 + lane;
-		const bool add = p.beta != 0.0f and row < p.M;
+		const T *old = reinterpret_cast<const T*>(p.c) + static_cast<long long>(row0 + lane) * p.N + column0;
+		const int old_columns = (ADD and row0 + lane < p.M) ? p.N - column0 : 0;
 #pragma unroll
 		for (int j = 0; j < kColumns / kPerPiece; j++)
 		{
 			float x[kPerPiece];
 #pragma unroll
-			for (int i = 0; i < kPerPiece; i += 2)
-			{
+			for (int i = 0; i < kPerPiece; i++)
 				x[i] = p.alpha * acc[j * kPerPiece + i];
-				x[i + 1] = p.alpha * acc[j * kPerPiece + i + 1];
-			}
-			if (add)
+			if (ADD and j * kPerPiece < old_columns)
 			{
+				if (bulk) /* rows and pieces on 16-byte boundaries, whole pieces only */
+				{
+					const Vec<T, kPerPiece> v = load_vec<T, kPerPiece>(old + j * kPerPiece);
 #pragma unroll
-				for (int i = 0; i < kPerPiece; i++)
-					if (column0 + j * kPerPiece + i < p.N)
-						x[i] = fmaf(p.beta, load_c(p, row * p.N + column0 + j * kPerPiece + i), x[i]);
+					for (int i = 0; i < kPerPiece; i++)
+						x[i] = fmaf(p.beta, to_compute(v.v[i]), x[i]);
+				}
+				else
+				{
+#pragma unroll
+					for (int i = 0; i < kPerPiece; i++)
+						if (j * kPerPiece + i < old_columns)
+							x[i] = fmaf(p.beta, to_compute(old[j * kPerPiece + i]), x[i]);
+				}
 			}
-			uint4 piece;
-			if constexpr (WIDE)
-				piece = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-			else
-				piece = make_uint4(pack_two(p.c_type, x[0], x[1]), pack_two(p.c_type, x[2], x[3]), pack_two(p.c_type, x[4], x[5]), pack_two(p.c_type, x[6], x[7]));
-			*reinterpret_cast<uint4*>(buffer + lane * 128 + ((j ^ (lane & 7)) << 4)) = piece;
+			Vec<T, kPerPiece> piece;
+#pragma unroll
+			for (int i = 0; i < kPerPiece; i++)
+				piece.v[i] = from_compute<T>(x[i]);
+			store_vec<T, kPerPiece>(reinterpret_cast<T*>(buffer + lane * 128 + ((j ^ (lane & 7)) << 4)), piece);
 		}
 		if (bulk)
 		{
@@ -538,20 +544,27 @@ namespace
 				for (int i = 0; i < kColumns / 32; i++)
 				{
 					const int column = i * 32 + lane;
-					const uint8_t *at = buffer + r * 128 + (((column / kPerPiece) ^ (r & 7)) << 4);
-					const long long to = static_cast<long long>(row0 + r) * p.N + column0 + column;
 					if (column0 + column < p.N)
-					{
-						if constexpr (WIDE)
-							reinterpret_cast<float*>(p.c)[to] = reinterpret_cast<const float*>(at)[column % kPerPiece];
-						else
-							reinterpret_cast<uint16_t*>(p.c)[to] = reinterpret_cast<const uint16_t*>(at)[column % kPerPiece];
-					}
+						reinterpret_cast<T*>(p.c)[static_cast<long long>(row0 + r) * p.N + column0 + column] =
+								reinterpret_cast<const T*>(buffer + r * 128 + (((column / kPerPiece) ^ (r & 7)) << 4))[column % kPerPiece];
 				}
 			__syncwarp();
 		}
 	}
+	/* a warp's 32 x 128 results through two buffers in turn */
+	template<typename T, bool ADD>
+	__device__ __forceinline__ void store_rows(const ScaledGemm &p, const CUtensorMap *mapC, uint8_t *buffers, const float (&acc)[128], int row0, int column0, int lane,
+			bool bulk)
+	{
+		constexpr int kColumns = 128 / static_cast<int>(sizeof(T));
+#pragma unroll
+		for (int sub = 0; sub < 128 / kColumns; sub++)
+			store_sub_tile<T, ADD>(p, mapC, buffers + (sub & 1) * kSubBytes, acc + sub * kColumns, row0, column0 + sub * kColumns, lane, bulk);
+	}
 
+	/* ADD: beta is not 0.  The type of C and this are template parameters because the store runs once per tile, out of a cold
+	 * instruction cache: every path that is not there is one that is not fetched. */
+	template<typename T, bool ADD>
 	__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) kernel_gemm_f8_pair(const __grid_constant__ CUtensorMap mapA,
 			const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapC, ScaledGemm p, int mBlocks, int nBlocks, int numTiles, int bulkStore,
 			int *deviceStatus)
@@ -561,8 +574,8 @@ namespace
 
 		__shared__ __align__(8) uint64_t full_bar[kPairStages];
 		__shared__ __align__(8) uint64_t empty_bar[kPairStages];
-		__shared__ __align__(8) uint64_t part_full_bar[4];
-		__shared__ __align__(8) uint64_t part_empty_bar[4];
+		__shared__ __align__(8) uint64_t part_full_bar[2];
+		__shared__ __align__(8) uint64_t part_empty_bar[2];
 		__shared__ __align__(8) uint64_t scale_free_bar[kScaleSlots];
 		__shared__ uint32_t tmem_base_slot;
 		__shared__ int abort_flag;
@@ -583,10 +596,10 @@ namespace
 				umma::mbar_init(&full_bar[s], 1);
 				umma::mbar_init(&empty_bar[s], 1);
 			}
-			for (int b = 0; b < 4; b++)
+			for (int b = 0; b < 2; b++)
 			{
 				umma::mbar_init(&part_full_bar[b], 2);
-				umma::mbar_init(&part_empty_bar[b], 2 * 4);
+				umma::mbar_init(&part_empty_bar[b], 2 * 8);
 			}
 			for (int b = 0; b < kScaleSlots; b++)
 				umma::mbar_init(&scale_free_bar[b], 8);
@@ -653,7 +666,7 @@ namespace
 			if (lane == 0 and rank == 0)
 			{
 				/* issuer b takes the blocks b, b + 2, ... of the whole sequence of tiles, whose slots are two apart */
-				constexpr uint32_t idesc = umma::make_instr_desc(umma::kAccumF32, umma::kFormatE4M3, umma::kFormatE4M3, false, false, 256, 128);
+				constexpr uint32_t idesc = umma::make_instr_desc(umma::kAccumF32, umma::kFormatE4M3, umma::kFormatE4M3, false, false, 256, 256);
 				const uint64_t desc0 = umma::make_smem_desc(umma::smem_u32(smem), 16, 1024, umma::kSwizzle128B);
 				const int b = warp - 1;
 				const int tiles = (numTiles - pair + pairs - 1) / pairs;
@@ -669,22 +682,16 @@ namespace
 						break;
 					}
 					const uint64_t desc = desc0 + static_cast<uint64_t>(stage * (kPairSlotBytes / 16));
-#pragma unroll
-					for (int h = 0; h < 2; h++)
+					if (not umma::mbar_wait(&part_empty_bar[b], part_phase ^ 1u, abort_ptr))
 					{
-						if (not umma::mbar_wait(&part_empty_bar[2 * b + h], part_phase ^ 1u, abort_ptr))
-						{
-							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorMmaWait);
-							ok = false;
-							break;
-						}
-						umma::tcgen05_fence_after();
-						/* rows h * 64 .. h * 64 + 63 of each CTA's half of B */
-						umma::mma_f8_pair_k4(tmem_base + static_cast<uint32_t>((2 * b + h) * 128), desc, desc + (kBlockBytes + h * 64 * 128) / 16, idesc, false);
-						if (h == 1)
-							umma::mma_commit_pair(&empty_bar[stage], 3);
-						umma::mma_commit_pair(&part_full_bar[2 * b + h], 3); /* the last one: who has seen it need not expect another arrival */
+						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorMmaWait);
+						ok = false;
+						break;
 					}
+					umma::tcgen05_fence_after();
+					umma::mma_f8_pair_k4(tmem_base + static_cast<uint32_t>(b * 256), desc, desc + kBlockBytes / 16, idesc, false);
+					umma::mma_commit_pair(&empty_bar[stage], 3);
+					umma::mma_commit_pair(&part_full_bar[b], 3); /* last: who has seen it need not expect another arrival */
 					part_phase ^= 1u;
 					stage += 2;
 					if (stage >= kPairStages)
@@ -699,7 +706,7 @@ namespace
 		{
 			/* Scales of this CTA's 128 rows and of the two column halves, four rows per lane, loaded kScaleAhead blocks before they are
 			 * handed over.  Block i may use slot i % 3 once every promotion warp has read block i - 3 (scale_free), and may arrive on
-			 * its accumulators' barriers once the phase of block i - 2 is over; both lie a block's time back, so that this warp is never
+			 * its accumulator's barrier once the phase of block i - 2 is over; both lie a block's time back, so that this warp is never
 			 * the one that is waited for. */
 			float ahead_a[kScaleAhead][4], ahead_b[kScaleAhead];
 			const int tiles = (numTiles - pair + pairs - 1) / pairs;
@@ -740,10 +747,10 @@ namespace
 					const long long i = i0 + d;
 					if (i >= total)
 						break;
-					uint64_t *bars = &part_full_bar[(i & 1) * 2];
+					uint64_t *bar = &part_full_bar[i & 1];
 					const uint32_t phase = (static_cast<uint32_t>(i >> 1) & 1u) ^ 1u;
 					ok = __all_sync(0xFFFFFFFFu, umma::mbar_wait(&scale_free_bar[d], slot_phase, abort_ptr)
-							and (i < 2 or (umma::mbar_wait(bars, phase, abort_ptr) and umma::mbar_wait(bars + 1, phase, abort_ptr))));
+							and (i < 2 or umma::mbar_wait(bar, phase, abort_ptr)));
 					if (not ok)
 					{
 						if (lane == 0)
@@ -756,8 +763,8 @@ namespace
 					if (lane < 2)
 						b_scale_s[d][lane] = ahead_b[d];
 					__syncwarp();
-					if (lane < 2)
-						umma::mbar_arrive(bars + lane);
+					if (lane == 0)
+						umma::mbar_arrive(bar);
 					fetch(ahead_a[d], ahead_b[d]);
 				}
 			}
@@ -766,8 +773,8 @@ namespace
 		{
 			asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairPromoteRegisters));
 			const int quarter = warp % 4;
-			const int half = (warp - kPairControlThreads / 32) / 4;
-			const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * 128);
+			const int column_half = (warp - kPairControlThreads / 32) / 4;
+			const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(column_half * 128);
 			uint8_t *buffers = smem + kPairStages * kPairSlotBytes + (warp - kPairControlThreads / 32) * 2 * kSubBytes;
 			uint32_t b = 0, phase = 0, slot = 0;
 			bool ok = true;
@@ -775,16 +782,14 @@ namespace
 			{
 				const PairTile t = pair_tile(tile, mBlocks, nBlocks);
 				const int row0 = t.m * 256 + rank * 128 + quarter * 32;
-				/* columns 0..63 of this warp's accumulator come from the first CTA's rows of B, 64..127 from the second's */
-				const int column0 = t.n * 256 + half * 64;
+				const int column0 = t.n * 256 + column_half * 128;
 				float acc[128];
 #pragma unroll
 				for (int i = 0; i < 128; i++)
 					acc[i] = 0.0f;
 				for (int kb = 0; kb < p.blocks; kb++)
 				{
-					uint64_t *bar = &part_full_bar[2 * b + half];
-					ok = __all_sync(0xFFFFFFFFu, lane != 0 or umma::mbar_wait(bar, phase, abort_ptr)); /* one lane polls: 590 -> 540 us at 8192^3 */
+					ok = __all_sync(0xFFFFFFFFu, lane != 0 or umma::mbar_wait(&part_full_bar[b], phase, abort_ptr)); /* one lane polls: 590 -> 540 us at 8192^3 */
 					if (not ok)
 					{
 						if (lane == 0)
@@ -795,8 +800,7 @@ namespace
 					const uint32_t from = lanes + b * 256u;
 					uint32_t r[2][16];
 					umma::tmem_load_32x16(from, r[0]);
-					const float a_scale = a_scale_s[slot][quarter * 32 + lane];
-					const float scale[2] = { a_scale * b_scale_s[slot][0], a_scale * b_scale_s[slot][1] };
+					const float scale = a_scale_s[slot][quarter * 32 + lane] * b_scale_s[slot][column_half];
 					__syncwarp();
 					if (lane == 0)
 						umma::mbar_arrive(&scale_free_bar[slot]);
@@ -812,29 +816,18 @@ namespace
 							umma::tcgen05_fence_before();
 							__syncwarp();
 							if (lane == 0)
-								umma::mbar_arrive_cluster_relaxed(umma::map_to_cta(umma::smem_u32(&part_empty_bar[2 * b + half]), 0));
+								umma::mbar_arrive_cluster_relaxed(umma::map_to_cta(umma::smem_u32(&part_empty_bar[b]), 0));
 						}
 #pragma unroll
 						for (int i = 0; i < 16; i++)
-							acc[chunk * 16 + i] = fmaf(__uint_as_float(r[chunk & 1][i]), scale[chunk / 4], acc[chunk * 16 + i]);
+							acc[chunk * 16 + i] = fmaf(__uint_as_float(r[chunk & 1][i]), scale, acc[chunk * 16 + i]);
 					}
 					if ((b ^= 1u) == 0)
 						phase ^= 1u;
 				}
 				if (not ok)
 					break;
-				if (p.c_type == AVOCADO_DTYPE_FLOAT32)
-				{
-#pragma unroll
-					for (int sub = 0; sub < 4; sub++)
-						store_sub_tile<true>(p, &mapC, buffers + (sub & 1) * kSubBytes, acc + sub * 32, row0, column0 + (sub / 2) * 128 + (sub % 2) * 32, lane, bulkStore != 0);
-				}
-				else
-				{
-#pragma unroll
-					for (int sub = 0; sub < 2; sub++)
-						store_sub_tile<false>(p, &mapC, buffers + sub * kSubBytes, acc + sub * 64, row0, column0 + sub * 128, lane, bulkStore != 0);
-				}
+				store_rows<T, ADD>(p, &mapC, buffers, acc, row0, column0, lane, bulkStore != 0);
 			}
 			if (lane == 0)
 				umma::tma_store_wait_all<0>();
@@ -936,9 +929,10 @@ namespace
 		return launch_split<128, LOADERS>(ctx, p);
 	}
 
+	template<typename T, bool ADD>
 	avStatus_t launch_pair(ContextObject &ctx, const ScaledGemm &p)
 	{
-		auto kernel = kernel_gemm_f8_pair;
+		auto kernel = kernel_gemm_f8_pair<T, ADD>;
 		static PerDeviceOnce configured;
 		if (configured.run(ctx.device, [&]() -> cudaError_t { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes); }) != cudaSuccess)
 		{
@@ -948,7 +942,7 @@ namespace
 		CUtensorMap mapA, mapB, mapC = { };
 		if (not make_operand_map(&mapA, p.a, p.M, p.K, 128) or not make_operand_map(&mapB, p.b, p.N, p.K, 128))
 			return AVOCADO_STATUS_INTERNAL_ERROR;
-		const int size = p.c_type == AVOCADO_DTYPE_FLOAT32 ? 4 : 2;
+		constexpr int size = static_cast<int>(sizeof(T));
 		const bool bulk = static_cast<long long>(p.N) * size % 16 == 0 and reinterpret_cast<uintptr_t>(p.c) % 16 == 0;
 		if (bulk)
 		{
@@ -968,6 +962,16 @@ namespace
 		const cudaError_t launched = launch_chained(kernel, dim3(2 * pairs), dim3(kPairThreads), kPairSmemBytes, ctx.getStream(), mapA, mapB, mapC, p, m_blocks,
 				n_blocks, static_cast<int>(tiles), bulk ? 1 : 0, ctx.getDeviceStatus());
 		return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
+	}
+
+	avStatus_t launch_pair(ContextObject &ctx, const ScaledGemm &p)
+	{
+		const bool add = p.beta != 0.0f;
+		if (p.c_type == AVOCADO_DTYPE_FLOAT32)
+			return add ? launch_pair<float, true>(ctx, p) : launch_pair<float, false>(ctx, p);
+		if (p.c_type == AVOCADO_DTYPE_FLOAT16)
+			return add ? launch_pair<half, true>(ctx, p) : launch_pair<half, false>(ctx, p);
+		return add ? launch_pair<__nv_bfloat16, true>(ctx, p) : launch_pair<__nv_bfloat16, false>(ctx, p);
 	}
 
 	avStatus_t launch(ContextObject &ctx, const ScaledGemm &p)
