@@ -984,7 +984,7 @@ namespace
 			return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
 		}
 		const bool tma = p.K % 16 == 0 and (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0;
-		if (tma and static_cast<long long>((p.M + 255) / 256) * ((p.N + 255) / 256) >= 32)
+		if (tma and p.M > 128 and static_cast<long long>((p.M + 255) / 256) * ((p.N + 255) / 256) >= 32)
 			return launch_pair(ctx, p);
 		return tma ? launch_split<false>(ctx, p) : launch_split<true>(ctx, p);
 	}

@@ -65,6 +65,35 @@ namespace
 	{
 		return VEC ? first + l * kPerLane + i : first + l + i * kLanes;
 	}
+	/* the same as they are stored, for kernels that hold many at once; positions past the end hold zeros */
+	template<bool VEC, typename T>
+	__device__ __forceinline__ void load_eight(Vec<T, kPerLane> &v, const T *row, int first, int l, int columns)
+	{
+#pragma unroll
+		for (int i = 0; i < kPerLane; i++)
+			v.v[i] = from_compute<T>(0.0f);
+		if constexpr (VEC)
+		{
+			const int column = first + l * kPerLane;
+			if (column < columns)
+			{
+				constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
+#pragma unroll
+				for (int j = 0; j < kPerLane; j += kPiece)
+					*reinterpret_cast<Vec<T, kPiece>*>(&v.v[j]) = load_vec<T, kPiece>(row + column + j);
+			}
+		}
+		else
+		{
+#pragma unroll
+			for (int i = 0; i < kPerLane; i++)
+			{
+				const int column = column_of<VEC>(first, l, i);
+				if (column < columns)
+					v.v[i] = row[column];
+			}
+		}
+	}
 	template<bool VEC, typename T>
 	__device__ __forceinline__ void load_eight(float (&v)[kPerLane], const T *row, int first, int l, int columns)
 	{
@@ -160,29 +189,116 @@ namespace
 		return __uint_as_float(bits);
 	}
 
-	/* ---- 1 x 128 blocks: half a warp per block, no block-wide step ------------------------------------------------ */
+	/* The largest magnitude of raw elements as an integer; two 16-bit patterns are compared at once. */
+	__device__ __forceinline__ uint32_t raw_max(const Vec<float, kPerLane> &v, uint32_t bits)
+	{
+#pragma unroll
+		for (int i = 0; i < kPerLane; i++)
+			bits = max(bits, magnitude_bits(v.v[i]));
+		return bits;
+	}
+	template<typename T>
+	__device__ __forceinline__ uint32_t raw_max(const Vec<T, kPerLane> &v, uint32_t bits)
+	{
+		const uint32_t *pairs = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+		for (int i = 0; i < kPerLane / 2; i++)
+			bits = __vmaxu2(bits, pairs[i] & 0x7FFF7FFFu);
+		return bits;
+	}
+	/* over the lanes that differ in the bits below `lanes`, as a clamped float */
+	template<typename T, int LANES>
+	__device__ __forceinline__ uint32_t raw_max_over_lanes(uint32_t bits)
+	{
+#pragma unroll
+		for (int i = LANES / 2; i > 0; i /= 2)
+		{
+			const uint32_t other = __shfl_xor_sync(kFullWarp, bits, i);
+			bits = sizeof(T) == 4 ? max(bits, other) : __vmaxu2(bits, other);
+		}
+		return bits;
+	}
+	template<typename T>
+	__device__ __forceinline__ uint32_t float_bits(uint32_t bits) /* of the larger half */
+	{
+		if constexpr (sizeof(T) == 4)
+			return bits;
+		else
+		{
+			const uint16_t largest = static_cast<uint16_t>(max(bits & 0xFFFFu, bits >> 16));
+			return __float_as_uint(to_compute(*reinterpret_cast<const T*>(&largest)));
+		}
+	}
+	template<bool VEC, typename T>
+	__device__ __forceinline__ void store_codes(uint8_t *row, const Vec<T, kPerLane> &v, float r, int first, int l, int columns)
+	{
+		float x[kPerLane];
+#pragma unroll
+		for (int i = 0; i < kPerLane; i++)
+			x[i] = to_compute(v.v[i]);
+		store_codes<VEC>(row, x, r, first, l, columns);
+	}
+
+	/* ---- 1 x 128 blocks: half a warp per block, no block-wide step ------------------------------------------------
+	 * A half-warp takes kAtOnce blocks, one after every sixteenth, and requests all of them before it works on the first, so that
+	 * an SM has 64 KB (16-bit) on the way; positions advance by addition, the only division is the first. */
+	constexpr int kAtOnce = 4;
+	constexpr int kHalfWarps = kThreads / kLanes;
+
+	struct BlockAt
+	{
+			long long row;
+			int block;
+
+			__device__ __forceinline__ void advance(long long rows, int step, int blocks)
+			{
+				row += rows;
+				block += step;
+				if (block >= blocks)
+				{
+					block -= blocks;
+					row++;
+				}
+			}
+	};
+
 	template<typename T, bool VEC>
 	__global__ void __launch_bounds__(kThreads) kernel_quantize_rows(const T *__restrict__ x, uint8_t *__restrict__ y, float *__restrict__ scales,
-			long long total, int columns, int blocks)
+			long long total, int columns, int blocks, long long strideRows, int strideBlocks)
 	{
 		chain_release();
 		chain_wait();
 		const int l = threadIdx.x % kLanes;
-		const long long stride = static_cast<long long>(gridDim.x) * (kThreads / kLanes);
-		for (long long first = static_cast<long long>(blockIdx.x) * (kThreads / kLanes); first < total; first += stride)
+		long long b = static_cast<long long>(blockIdx.x) * (kHalfWarps * kAtOnce) + threadIdx.x / kLanes;
+		BlockAt at;
+		at.row = b / blocks;
+		at.block = static_cast<int>(b - at.row * blocks);
+		const int next_rows = kHalfWarps / blocks, next_blocks = kHalfWarps % blocks;
+		for (long long first = b - threadIdx.x / kLanes; first < total; first += static_cast<long long>(gridDim.x) * (kHalfWarps * kAtOnce))
 		{
-			const long long b = first + threadIdx.x / kLanes;
-			const bool inside = b < total;
-			const long long row = inside ? b / blocks : 0;
-			const int column = inside ? static_cast<int>(b - row * blocks) * kScaleBlock : columns;
-			float v[kPerLane];
-			load_eight<VEC>(v, x + row * columns, column, l, columns);
-			uint32_t bits = 0;
-			largest_magnitude(v, bits);
-			const float amax = clamped_amax(max_over_half_warp(bits));
-			store_codes<VEC>(y + row * columns, v, kLargestE4m3 / amax, column, l, columns);
-			if (inside and l == 0)
-				scales[b] = amax / kLargestE4m3;
+			Vec<T, kPerLane> v[kAtOnce];
+			long long offset[kAtOnce];
+			int column[kAtOnce];
+			BlockAt a = at;
+#pragma unroll
+			for (int i = 0; i < kAtOnce; i++)
+			{
+				const bool inside = b + i * kHalfWarps < total;
+				offset[i] = inside ? a.row * columns : 0;
+				column[i] = inside ? a.block * kScaleBlock : columns;
+				load_eight<VEC>(v[i], x + offset[i], column[i], l, columns);
+				a.advance(next_rows, next_blocks, blocks);
+			}
+#pragma unroll
+			for (int i = 0; i < kAtOnce; i++)
+			{
+				const float amax = clamped_amax(float_bits<T>(raw_max_over_lanes<T, kLanes>(raw_max(v[i], 0u))));
+				store_codes<VEC>(y + offset[i], v[i], kLargestE4m3 / amax, column[i], l, columns);
+				if (l == 0 and column[i] < columns)
+					scales[b + i * kHalfWarps] = amax / kLargestE4m3;
+			}
+			b += static_cast<long long>(gridDim.x) * (kHalfWarps * kAtOnce);
+			at.advance(strideRows, strideBlocks, blocks);
 		}
 	}
 
@@ -203,7 +319,7 @@ namespace
 			const long long block_row = b / blocks;
 			const int column = static_cast<int>(b - block_row * blocks) * kScaleBlock;
 			const long long row0 = block_row * kScaleBlock + threadIdx.x / kLanes;
-			float v[kPasses][kPerLane];
+			Vec<T, kPerLane> v[kPasses];
 			uint32_t bits = 0;
 #pragma unroll
 			for (int p = 0; p < kPasses; p++)
@@ -213,8 +329,8 @@ namespace
 			}
 #pragma unroll
 			for (int p = 0; p < kPasses; p++)
-				largest_magnitude(v[p], bits);
-			bits = __reduce_max_sync(kFullWarp, bits);
+				bits = raw_max(v[p], bits);
+			bits = float_bits<T>(raw_max_over_lanes<T, 32>(bits));
 			if (threadIdx.x % 32 == 0)
 				warp_max[turn][threadIdx.x / 32] = bits;
 			__syncthreads(); /* two sets of slots: the next turn's writes cannot meet this turn's reads */
@@ -236,21 +352,18 @@ namespace
 	}
 
 	/* ---- norm + quantise ------------------------------------------------------------------------------------------------
-	 * `warps` warps (a power of two) share a row; half-warp i of them owns the blocks i, i + 2 * warps, ... .  ITEMS > 0: at most
-	 * ITEMS blocks per half-warp, kept in registers between the sum of squares and the codes.  ITEMS = 0: rows of any length,
-	 * read twice. */
+	 * `halves` half-warps (a power of two) share a row; number i of them owns the blocks i, i + halves, ... .  ITEMS > 0: at most
+	 * ITEMS blocks each, kept in registers between the sum of squares and the codes.  ITEMS = 0: rows of any length, read twice. */
 	template<typename T, int ITEMS, bool VEC>
 	__global__ void __launch_bounds__(1024) kernel_rms_norm_quantize(const T *x, const T *z, T *h, const float *__restrict__ gamma, uint8_t *__restrict__ y,
-			float *__restrict__ scales, long long rows, int columns, int blocks, int warps, float epsilon)
+			float *__restrict__ scales, long long rows, int columns, int blocks, int halves, float epsilon)
 	{
 		__shared__ float warp_sum[32];
 		chain_release();
 		chain_wait();
-		const int warp = threadIdx.x / 32;
 		const int l = threadIdx.x % kLanes;
-		const int warp_in_row = warp & (warps - 1);
-		const int half = warp_in_row * 2 + (threadIdx.x % 32) / kLanes;
-		const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / (32 * warps)) + warp / warps;
+		const int half = (threadIdx.x / kLanes) & (halves - 1);
+		const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / kLanes / halves) + threadIdx.x / kLanes / halves;
 		const bool inside = row < rows;
 		const int limit = inside ? columns : 0; /* a row past the end has no columns: nothing is read or written for it */
 		const long long offset = inside ? row * columns : 0;
@@ -267,13 +380,11 @@ namespace
 					v[i] += other[i];
 			}
 		};
-		auto finish = [&](float (&v)[kPerLane], int b, float rstd)
+		auto finish = [&](float (&v)[kPerLane], const float (&g)[kPerLane], int b, float rstd)
 		{
 			const int column = b * kScaleBlock;
 			if (h != nullptr)
 				store_eight<VEC>(h + offset, v, column, l, limit);
-			float g[kPerLane];
-			load_eight<VEC>(g, gamma, column, l, limit);
 			uint32_t bits = 0;
 #pragma unroll
 			for (int i = 0; i < kPerLane; i++)
@@ -293,20 +404,23 @@ namespace
 		};
 
 		constexpr int kHeld = ITEMS > 0 ? ITEMS : 1;
-		float v[kHeld][kPerLane];
+		constexpr bool kGammaFirst = ITEMS == 1; /* a row per block: gamma's latency is hidden behind the row's, not added to it */
+		float v[kHeld][kPerLane], g[kPerLane];
 		float sum = 0.0f;
 		if constexpr (ITEMS > 0)
 		{
 #pragma unroll
 			for (int i = 0; i < kHeld; i++)
-				load_sum(v[i], (half + i * 2 * warps) * kScaleBlock);
+				load_sum(v[i], (half + i * halves) * kScaleBlock);
+			if constexpr (kGammaFirst)
+				load_eight<VEC>(g, gamma, half * kScaleBlock, l, limit);
 #pragma unroll
 			for (int i = 0; i < kHeld; i++)
 				sum = square_sum(v[i], sum);
 		}
 		else
 		{
-			for (int b = half; b < blocks; b += 2 * warps)
+			for (int b = half; b < blocks; b += halves)
 			{
 				load_sum(v[0], b * kScaleBlock);
 				sum = square_sum(v[0], sum);
@@ -314,31 +428,39 @@ namespace
 			__syncwarp();
 		}
 #pragma unroll
-		for (int i = 16; i > 0; i /= 2)
+		for (int i = kLanes / 2; i > 0; i /= 2)
 			sum += __shfl_xor_sync(kFullWarp, sum, i);
-		if (warps > 1)
+		if (halves > 1)
+			sum += __shfl_xor_sync(kFullWarp, sum, kLanes);
+		if (halves > 2)
 		{
+			const int warp = threadIdx.x / 32, warps = halves / 2;
 			if (threadIdx.x % 32 == 0)
 				warp_sum[warp] = sum;
 			__syncthreads();
 			sum = 0.0f;
 			for (int w = 0; w < warps; w++) /* the same order in every thread of the row */
-				sum += warp_sum[warp - warp_in_row + w];
+				sum += warp_sum[(warp & ~(warps - 1)) + w];
 		}
 		const float rstd = 1.0f / sqrtf(sum / static_cast<float>(columns) + epsilon);
 		if constexpr (ITEMS > 0)
 		{
 #pragma unroll
 			for (int i = 0; i < kHeld; i++)
-				finish(v[i], half + i * 2 * warps, rstd);
+			{
+				if constexpr (not kGammaFirst)
+					load_eight<VEC>(g, gamma, (half + i * halves) * kScaleBlock, l, limit);
+				finish(v[i], g, half + i * halves, rstd);
+			}
 		}
 		else
 		{
 			/* both half-warps of a warp go round equally often: the maximum is taken with all lanes present */
-			for (int b = half; b - (half & 1) < blocks; b += 2 * warps)
+			for (int b = half; b - (half & 1) < blocks; b += halves)
 			{
 				load_sum(v[0], b * kScaleBlock);
-				finish(v[0], b, rstd);
+				load_eight<VEC>(g, gamma, b * kScaleBlock, l, limit);
+				finish(v[0], g, b, rstd);
 			}
 		}
 	}
@@ -368,10 +490,13 @@ namespace
 		else
 		{
 			const long long total = rows * blocks;
-			const long long wanted = (total + kThreads / kLanes - 1) / (kThreads / kLanes);
-			const dim3 grid(static_cast<unsigned>(std::min<long long>(wanted, static_cast<long long>(sm_count(ctx)) * 8)));
+			constexpr int kPerBlock = kHalfWarps * kAtOnce;
+			const long long wanted = (total + kPerBlock - 1) / kPerBlock;
+			const dim3 grid(static_cast<unsigned>(std::min<long long>(wanted, 1 << 30)));
+			const long long stride = static_cast<long long>(grid.x) * kPerBlock;
 			auto kernel = vec ? kernel_quantize_rows<T, true> : kernel_quantize_rows<T, false>;
-			launched = launch_chained(kernel, grid, dim3(kThreads), 0, ctx.getStream(), xp, y.ptr, sp, total, columns, blocks);
+			launched = launch_chained(kernel, grid, dim3(kThreads), 0, ctx.getStream(), xp, y.ptr, sp, total, columns, blocks, stride / blocks,
+					static_cast<int>(stride % blocks));
 		}
 		return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
 	}
@@ -387,24 +512,23 @@ namespace
 	avStatus_t launch_norm(ContextObject &ctx, const NormArgs &a)
 	{
 		const int blocks = scale_blocks(a.columns);
-		/* Warps per row: enough that a half-warp holds at most four blocks; when the rows alone do not fill the machine, as many
-		 * as there are pairs of blocks, because then the time of one row is the time of the call. */
-		const bool few_rows = a.rows < 2 * sm_count(ctx);
-		const int wanted = few_rows ? (blocks + 1) / 2 : (blocks + 7) / 8;
-		int warps = 1;
-		while (warps < wanted and warps < 32)
-			warps *= 2;
-		const int per_half = (blocks + 2 * warps - 1) / (2 * warps);
-		const int threads = std::max(32 * warps, few_rows ? 32 : kThreads);
-		const long long rows_per_block = threads / (32 * warps);
+		/* Half-warps per row: enough that each holds at most four blocks; while the rows do not fill the machine, as many as there are
+		 * blocks, because then the time of one row is the time of the call. */
+		int halves = 1;
+		const long long room = static_cast<long long>(sm_count(ctx)) * (1024 / kLanes);
+		while (halves < 64 and halves < blocks and ((blocks + halves - 1) / halves > 4 or a.rows * halves * 2 <= room))
+			halves *= 2;
+		const int per_half = (blocks + halves - 1) / halves;
+		const int threads = std::max(kLanes * halves, kThreads);
+		const long long rows_per_block = threads / (kLanes * halves);
 		const long long grid = (a.rows + rows_per_block - 1) / rows_per_block;
 		if (grid > 0x7FFFFFFFll)
 			return AVOCADO_STATUS_NOT_SUPPORTED;
 		auto kernel = per_half <= 1 ? kernel_rms_norm_quantize<T, 1, VEC> : per_half <= 2 ? kernel_rms_norm_quantize<T, 2, VEC> :
-				per_half <= 4 ? kernel_rms_norm_quantize<T, 4, VEC> : kernel_rms_norm_quantize<T, 0, VEC>;
+				per_half <= 3 ? kernel_rms_norm_quantize<T, 3, VEC> : per_half <= 4 ? kernel_rms_norm_quantize<T, 4, VEC> : kernel_rms_norm_quantize<T, 0, VEC>;
 		const cudaError_t launched = launch_chained(kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, ctx.getStream(),
 				reinterpret_cast<const T*>(a.x.ptr), reinterpret_cast<const T*>(a.z.ptr), reinterpret_cast<T*>(a.h.ptr), reinterpret_cast<const float*>(a.gamma.ptr),
-				a.y.ptr, reinterpret_cast<float*>(a.scales.ptr), a.rows, a.columns, blocks, warps, a.epsilon);
+				a.y.ptr, reinterpret_cast<float*>(a.scales.ptr), a.rows, a.columns, blocks, halves, a.epsilon);
 		return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
 	}
 	template<typename T>
