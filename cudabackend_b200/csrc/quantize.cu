@@ -409,9 +409,22 @@ namespace
 		float sum = 0.0f;
 		if constexpr (ITEMS > 0)
 		{
+			{
+				/* every load is requested before the first is used */
+				Vec<T, kPerLane> rx[kHeld], rz[kHeld];
 #pragma unroll
-			for (int i = 0; i < kHeld; i++)
-				load_sum(v[i], (half + i * halves) * kScaleBlock);
+				for (int i = 0; i < kHeld; i++)
+				{
+					load_eight<VEC>(rx[i], x + offset, (half + i * halves) * kScaleBlock, l, limit);
+					if (z != nullptr)
+						load_eight<VEC>(rz[i], z + offset, (half + i * halves) * kScaleBlock, l, limit);
+				}
+#pragma unroll
+				for (int i = 0; i < kHeld; i++)
+#pragma unroll
+					for (int k = 0; k < kPerLane; k++)
+						v[i][k] = z != nullptr ? to_compute(rx[i].v[k]) + to_compute(rz[i].v[k]) : to_compute(rx[i].v[k]);
+			}
 			if constexpr (kGammaFirst)
 				load_eight<VEC>(g, gamma, half * kScaleBlock, l, limit);
 #pragma unroll
@@ -512,14 +525,17 @@ namespace
 	avStatus_t launch_norm(ContextObject &ctx, const NormArgs &a)
 	{
 		const int blocks = scale_blocks(a.columns);
-		/* Half-warps per row: enough that each holds at most four blocks; while the rows do not fill the machine, as many as there are
-		 * blocks, because then the time of one row is the time of the call. */
+		/* Half-warps per row: enough that each holds at most four blocks, or two where that makes 64 to 256 threads of a row (4096 x
+		 * 4096 bfloat16: 27 us with two, 29.5 with four; 8192 x 8192: 110 us with two, 102 with four; 50176 x 264: 26 with two, 17
+		 * with four).  While the rows do not fill the machine, as many as there are blocks, because then the time of one row is the
+		 * time of the call. */
+		const int most_items = (blocks > 4 and blocks <= 32) ? 2 : 4;
 		int halves = 1;
 		const long long room = static_cast<long long>(sm_count(ctx)) * (1024 / kLanes);
-		while (halves < 64 and halves < blocks and ((blocks + halves - 1) / halves > 4 or a.rows * halves * 2 <= room))
+		while (halves < 64 and halves < blocks and ((blocks + halves - 1) / halves > most_items or a.rows * halves * 2 <= room))
 			halves *= 2;
 		const int per_half = (blocks + halves - 1) / halves;
-		const int threads = std::max(kLanes * halves, kThreads);
+		const int threads = halves >= 8 ? kLanes * halves : kThreads; /* rows that meet at a barrier have a thread block to themselves */
 		const long long rows_per_block = threads / (kLanes * halves);
 		const long long grid = (a.rows + rows_per_block - 1) / rows_per_block;
 		if (grid > 0x7FFFFFFFll)
