@@ -129,8 +129,13 @@ namespace
 			static_assert(TOKENS * 512 <= kStages * kStageBytes, "the partial sums reuse the slots");
 			static constexpr int kWantedColumns = kStages * kPerStage * TOKENS;
 			static constexpr int kTmemColumns = kWantedColumns <= 128 ? 128 : kWantedColumns <= 256 ? 256 : 512;
+			/* promotion warps: four for the 128 lanes of TMEM, twice that where each would hold more than 32 tokens */
+			static constexpr int kPromoteWarps = TOKENS > 32 ? 8 : 4;
+			static constexpr int kPromoteThreads = kPromoteWarps * 32;
+			static constexpr int kTokensPerWarp = TOKENS / (kPromoteWarps / 4);
+			static constexpr int kMmaWarp = kPromoteWarps;
 			static constexpr int kLoaderThreads = LOADERS ? 128 : 32;
-			static constexpr int kThreads = 160 + kLoaderThreads;
+			static constexpr int kThreads = kPromoteThreads + 32 + kLoaderThreads;
 	};
 
 	/* 16 bytes from any address, zero past the first `valid`; only bytes inside [low, high) are touched */
@@ -180,7 +185,7 @@ namespace
 		__shared__ __align__(8) uint64_t drained_bar[kStages];
 		__shared__ uint32_t tmem_base_slot;
 		__shared__ int abort_flag;
-		__shared__ __align__(16) float scale_s[4][kPerStage * TOKENS];
+		__shared__ __align__(16) float scale_s[Cfg::kPromoteWarps][kPerStage * Cfg::kTokensPerWarp];
 
 		const int warp = threadIdx.x / 32;
 		const int lane = threadIdx.x % 32;
@@ -199,7 +204,7 @@ namespace
 			{
 				umma::mbar_init(&full_bar[s], LOADERS ? Cfg::kLoaderThreads : 1);
 				umma::mbar_init(&done_bar[s], 1);
-				umma::mbar_init(&drained_bar[s], 4);
+				umma::mbar_init(&drained_bar[s], Cfg::kPromoteWarps);
 			}
 			umma::mbar_fence_init();
 			if (not LOADERS)
@@ -208,7 +213,7 @@ namespace
 				umma::prefetch_tensormap(&mapB);
 			}
 		}
-		if (warp == 4)
+		if (warp == Cfg::kMmaWarp)
 		{
 			umma::tmem_alloc(&tmem_base_slot, Cfg::kTmemColumns);
 			umma::tmem_relinquish();
@@ -221,7 +226,7 @@ namespace
 		chain_release();
 		chain_wait();
 
-		if (warp == 4)
+		if (warp == Cfg::kMmaWarp)
 		{
 			if (lane == 0)
 			{
@@ -253,11 +258,11 @@ namespace
 				}
 			}
 		}
-		else if (warp > 4)
+		else if (warp > Cfg::kMmaWarp)
 		{
 			if (LOADERS or lane == 0)
 			{
-				const int thread = threadIdx.x - 160;
+				const int thread = threadIdx.x - Cfg::kPromoteThreads - 32;
 				int stage = 0;
 				uint32_t phase = 0;
 				for (int kb = first; kb < last; kb += kPerStage)
@@ -312,75 +317,88 @@ namespace
 		}
 		else
 		{
-			/* promotion: thread = row n0 + threadIdx.x of B, one accumulator per token */
-			float acc[TOKENS];
+			/* promotion: lane = row n0 + row of B, one accumulator per token of the warp's share */
+			constexpr int kTokens = Cfg::kTokensPerWarp;
+			constexpr int kScales = kPerStage * kTokens / 32; /* scales of a slot per lane */
+			static_assert(kPerStage * kTokens % 32 == 0 and kTokens % 16 == 0, "whole warps of scales, whole loads of TMEM");
+			const int row = warp % 4 * 32 + lane;
+			const int token0 = warp / 4 * kTokens;
+			float acc[kTokens];
 #pragma unroll
-			for (int t = 0; t < TOKENS; t++)
+			for (int t = 0; t < kTokens; t++)
 				acc[t] = 0.0f;
-			constexpr int kScales = kPerStage * TOKENS / 32; /* scales of a slot per lane */
-			float next[kScales];
-			auto fetch = [&](int kb)
+			/* the scales of the next two slots, as they come from memory: multiplied only when they are needed */
+			float next_a[2][kScales], next_b[2][kScales];
+			auto fetch = [&](float (&va)[kScales], float (&vb)[kScales], int kb)
 			{
 #pragma unroll
 				for (int i = 0; i < kScales; i++)
 				{
-					const int t = (i * 32 + lane) % TOKENS, g = kb + (i * 32 + lane) / TOKENS;
-					next[i] = 0.0f;
-					if (g < last and m0 + t < p.M)
-						next[i] = p.a_scale[static_cast<long long>(m0 + t) * p.blocks + g] * p.b_scale[static_cast<long long>(n_block) * p.blocks + g];
+					const int t = m0 + token0 + (i * 32 + lane) % kTokens, g = kb + (i * 32 + lane) / kTokens;
+					const bool inside = g < last and t < p.M;
+					va[i] = inside ? p.a_scale[static_cast<long long>(t) * p.blocks + g] : 0.0f;
+					vb[i] = inside ? p.b_scale[static_cast<long long>(n_block) * p.blocks + g] : 0.0f;
 				}
 			};
-			fetch(first);
-			const uint32_t lanes = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+			fetch(next_a[0], next_b[0], first);
+			fetch(next_a[1], next_b[1], first + kPerStage);
+			const uint32_t lanes = tmem_base + (static_cast<uint32_t>(warp % 4 * 32) << 16) + static_cast<uint32_t>(token0);
 			int stage = 0;
 			uint32_t phase = 0;
 			bool ok = true;
-			for (int kb = first; kb < last; kb += kPerStage)
+			for (int kb0 = first; kb0 < last and ok; kb0 += 2 * kPerStage)
 			{
-				__syncwarp(); /* the scales of the slot before have been read */
 #pragma unroll
-				for (int i = 0; i < kScales; i++)
-					scale_s[warp][i * 32 + lane] = next[i];
-				__syncwarp();
-				fetch(kb + kPerStage);
-				ok = __all_sync(0xFFFFFFFFu, umma::mbar_wait(&done_bar[stage], phase, abort_ptr));
-				if (not ok)
+				for (int u = 0; u < 2; u++)
 				{
-					if (lane == 0)
-						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
-					break;
-				}
-				umma::tcgen05_fence_after();
-#pragma unroll
-				for (int j = 0; j < kPerStage; j++)
-				{
-					if (kb + j >= last)
+					const int kb = kb0 + u * kPerStage;
+					if (kb >= last)
 						break;
+					__syncwarp(); /* the scales of the slot before have been read */
 #pragma unroll
-					for (int t0 = 0; t0 < TOKENS; t0 += 16)
+					for (int i = 0; i < kScales; i++)
+						scale_s[warp][i * 32 + lane] = next_a[u][i] * next_b[u][i];
+					__syncwarp();
+					fetch(next_a[u], next_b[u], kb + 2 * kPerStage);
+					ok = __all_sync(0xFFFFFFFFu, lane != 0 or umma::mbar_wait(&done_bar[stage], phase, abort_ptr));
+					if (not ok)
 					{
-						uint32_t r[16];
-						umma::tmem_load_32x16(lanes + static_cast<uint32_t>((stage * kPerStage + j) * TOKENS + t0), r);
-						umma::tmem_load_wait(r);
+						if (lane == 0)
+							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
+						break;
+					}
+					umma::tcgen05_fence_after();
 #pragma unroll
-						for (int t = 0; t < 16; t += 4)
+					for (int j = 0; j < kPerStage; j++)
+					{
+						if (kb + j >= last)
+							break;
+#pragma unroll
+						for (int t0 = 0; t0 < kTokens; t0 += 16)
 						{
-							const float4 s = *reinterpret_cast<const float4*>(&scale_s[warp][j * TOKENS + t0 + t]);
-							acc[t0 + t] = fmaf(__uint_as_float(r[t]), s.x, acc[t0 + t]);
-							acc[t0 + t + 1] = fmaf(__uint_as_float(r[t + 1]), s.y, acc[t0 + t + 1]);
-							acc[t0 + t + 2] = fmaf(__uint_as_float(r[t + 2]), s.z, acc[t0 + t + 2]);
-							acc[t0 + t + 3] = fmaf(__uint_as_float(r[t + 3]), s.w, acc[t0 + t + 3]);
+							uint32_t r[16];
+							umma::tmem_load_32x16(lanes + static_cast<uint32_t>((stage * kPerStage + j) * TOKENS + t0), r);
+							umma::tmem_load_wait(r);
+#pragma unroll
+							for (int t = 0; t < 16; t += 4)
+							{
+								const float4 s = *reinterpret_cast<const float4*>(&scale_s[warp][j * kTokens + t0 + t]);
+								acc[t0 + t] = fmaf(__uint_as_float(r[t]), s.x, acc[t0 + t]);
+								acc[t0 + t + 1] = fmaf(__uint_as_float(r[t + 1]), s.y, acc[t0 + t + 1]);
+								acc[t0 + t + 2] = fmaf(__uint_as_float(r[t + 2]), s.z, acc[t0 + t + 2]);
+								acc[t0 + t + 3] = fmaf(__uint_as_float(r[t + 3]), s.w, acc[t0 + t + 3]);
+							}
 						}
 					}
-				}
-				umma::tcgen05_fence_before();
-				__syncwarp();
-				if (lane == 0)
-					umma::mbar_arrive(&drained_bar[stage]);
-				if (++stage == kStages)
-				{
-					stage = 0;
-					phase ^= 1u;
+					umma::tcgen05_fence_before();
+					__syncwarp();
+					if (lane == 0)
+						umma::mbar_arrive(&drained_bar[stage]);
+					if (++stage == kStages)
+					{
+						stage = 0;
+						phase ^= 1u;
+					}
 				}
 			}
 			/* Every MMA of this CTA has run (this warp waited for the last one), and each of them had waited for its copies: the
@@ -389,8 +407,8 @@ namespace
 			{
 				float *partial = reinterpret_cast<float*>(smem);
 #pragma unroll
-				for (int t = 0; t < TOKENS; t++)
-					partial[t * 128 + threadIdx.x] = acc[t];
+				for (int t = 0; t < kTokens; t++)
+					partial[(token0 + t) * 128 + row] = acc[t];
 			}
 		}
 
@@ -399,11 +417,11 @@ namespace
 			umma::drain_after_abort();
 		if (splits > 1)
 			umma::cluster_sync_all(); /* the partial sums of every CTA are written */
-		if (warp < 4 and abort_flag == 0)
+		if (threadIdx.x < Cfg::kPromoteThreads and abort_flag == 0)
 		{
 			const int tokens = min(TOKENS, p.M - m0);
 			const uint32_t partial = umma::smem_u32(smem);
-			for (int i = rank * 128 + threadIdx.x; i < tokens * 32; i += splits * 128)
+			for (int i = rank * Cfg::kPromoteThreads + threadIdx.x; i < tokens * 32; i += splits * Cfg::kPromoteThreads)
 			{
 				const int n = i % 32 * 4;
 				float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -428,7 +446,7 @@ namespace
 		__syncthreads();
 		if (splits > 1)
 			umma::cluster_sync_all(); /* nobody leaves while its partial sums may still be read */
-		if (warp == 4)
+		if (warp == Cfg::kMmaWarp)
 		{
 			umma::tcgen05_fence_after();
 			umma::tmem_dealloc(tmem_base, Cfg::kTmemColumns);
