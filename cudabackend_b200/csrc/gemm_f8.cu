@@ -108,10 +108,11 @@ namespace
 	 * K are split over the CTAs of a cluster; their partial sums meet in distributed shared memory and are added in the order
 	 * of the ranks (no scratch memory, no atomics, the same bits every time).
 	 *
-	 * One ring of STAGES slots serves three roles: full (copy -> MMA), done (MMA -> promotion), drained (promotion -> copy).  Each
-	 * block of K has its own accumulator in TMEM, because its scales are applied outside the tensor core:
-	 * acc[t] += scale[t] * part[t] in float32 registers, thread = row of B.  PER_STAGE blocks share a slot, so that the thread
-	 * that issues the MMAs waits and commits once per PER_STAGE * 4 MMAs.
+	 * full[s] (copy -> MMA) and done[s] (MMA and scales -> promotion, and back to the copies: the slot may be filled again) go round
+	 * over the slots of shared memory, drained[b] (promotion -> MMA and scales) over the accumulators in TMEM.  Each block of K has
+	 * an accumulator of its own, because its scales are applied outside the tensor core: acc[t] += scale[t] * part[t] in float32
+	 * registers, lane = row of B.  Two blocks share a slot, so that every role waits once per eight MMAs.  A warp of its own loads
+	 * the scales, slots ahead of their use, and hands them to all promotion warps through shared memory.
 	 *
 	 * LOADERS: four warps fill the slots with plain loads instead of the TMA copies, for row pitches or addresses that are no
 	 * multiple of 16 bytes.
@@ -119,23 +120,24 @@ namespace
 	template<int TOKENS, bool LOADERS>
 	struct SplitConfig
 	{
-			static constexpr int kPerStage = TOKENS <= 64 ? 2 : 1;
-			static constexpr int kStages = 4;
+			static constexpr int kPerStage = 2;
+			static constexpr int kStages = TOKENS <= 64 ? 4 : 3;
+			static constexpr int kBuffers = kStages * kPerStage * TOKENS <= 512 ? kStages : 512 / (kPerStage * TOKENS); /* accumulator slots in TMEM */
 			static constexpr int kPairBytes = kBlockBytes + TOKENS * kScaleBlock;
 			static constexpr int kStageBytes = kPerStage * kPairBytes;
 			/* Two CTAs of different clusters never share an SM: each could wait for the TMEM of the other's neighbour. */
 			static constexpr int kSmemBytes = kStages * kStageBytes + 1024;
 			static_assert(kSmemBytes > 116 * 1024 and kSmemBytes <= 228 * 1024, "one CTA per SM");
 			static_assert(TOKENS * 512 <= kStages * kStageBytes, "the partial sums reuse the slots");
-			static constexpr int kWantedColumns = kStages * kPerStage * TOKENS;
+			static constexpr int kWantedColumns = kBuffers * kPerStage * TOKENS;
 			static constexpr int kTmemColumns = kWantedColumns <= 128 ? 128 : kWantedColumns <= 256 ? 256 : 512;
 			/* promotion warps: four for the 128 lanes of TMEM, twice that where each would hold more than 32 tokens */
 			static constexpr int kPromoteWarps = TOKENS > 32 ? 8 : 4;
 			static constexpr int kPromoteThreads = kPromoteWarps * 32;
 			static constexpr int kTokensPerWarp = TOKENS / (kPromoteWarps / 4);
-			static constexpr int kMmaWarp = kPromoteWarps;
+			static constexpr int kMmaWarp = kPromoteWarps, kScaleWarp = kPromoteWarps + 1;
 			static constexpr int kLoaderThreads = LOADERS ? 128 : 32;
-			static constexpr int kThreads = kPromoteThreads + 32 + kLoaderThreads;
+			static constexpr int kThreads = kPromoteThreads + 64 + kLoaderThreads;
 	};
 
 	/* 16 bytes from any address, zero past the first `valid`; only bytes inside [low, high) are touched */
@@ -182,10 +184,10 @@ namespace
 
 		__shared__ __align__(8) uint64_t full_bar[kStages];
 		__shared__ __align__(8) uint64_t done_bar[kStages];
-		__shared__ __align__(8) uint64_t drained_bar[kStages];
+		__shared__ __align__(8) uint64_t drained_bar[Cfg::kBuffers];
 		__shared__ uint32_t tmem_base_slot;
 		__shared__ int abort_flag;
-		__shared__ __align__(16) float scale_s[Cfg::kPromoteWarps][kPerStage * Cfg::kTokensPerWarp];
+		__shared__ __align__(16) float scale_s[Cfg::kBuffers][kPerStage * TOKENS];
 
 		const int warp = threadIdx.x / 32;
 		const int lane = threadIdx.x % 32;
@@ -203,9 +205,10 @@ namespace
 			for (int s = 0; s < kStages; s++)
 			{
 				umma::mbar_init(&full_bar[s], LOADERS ? Cfg::kLoaderThreads : 1);
-				umma::mbar_init(&done_bar[s], 1);
-				umma::mbar_init(&drained_bar[s], Cfg::kPromoteWarps);
+				umma::mbar_init(&done_bar[s], 2);
 			}
+			for (int b = 0; b < Cfg::kBuffers; b++)
+				umma::mbar_init(&drained_bar[b], Cfg::kPromoteWarps);
 			umma::mbar_fence_init();
 			if (not LOADERS)
 			{
@@ -232,10 +235,15 @@ namespace
 			{
 				constexpr uint32_t idesc = umma::make_instr_desc(umma::kAccumF32, umma::kFormatE4M3, umma::kFormatE4M3, false, false, 128, TOKENS);
 				const uint64_t desc0 = umma::make_smem_desc(umma::smem_u32(smem), 16, 1024, umma::kSwizzle128B);
-				int stage = 0;
-				uint32_t phase = 0;
+				int stage = 0, buffer = 0;
+				uint32_t phase = 0, buffer_phase = 0;
 				for (int kb = first; kb < last; kb += kPerStage)
 				{
+					if (not umma::mbar_wait(&drained_bar[buffer], buffer_phase ^ 1u, abort_ptr))
+					{
+						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorMmaWait);
+						break;
+					}
 					if (not umma::mbar_wait(&full_bar[stage], phase, abort_ptr))
 					{
 						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorTmaWait);
@@ -247,9 +255,14 @@ namespace
 						if (kb + j < last)
 						{
 							const uint64_t desc = desc0 + static_cast<uint64_t>((stage * Cfg::kStageBytes + j * Cfg::kPairBytes) / 16);
-							umma::mma_f8_k4(tmem_base + static_cast<uint32_t>((stage * kPerStage + j) * TOKENS), desc, desc + kBlockBytes / 16, idesc, false);
+							umma::mma_f8_k4(tmem_base + static_cast<uint32_t>((buffer * kPerStage + j) * TOKENS), desc, desc + kBlockBytes / 16, idesc, false);
 						}
 					umma::mma_commit(&done_bar[stage]);
+					if (++buffer == Cfg::kBuffers)
+					{
+						buffer = 0;
+						buffer_phase ^= 1u;
+					}
 					if (++stage == kStages)
 					{
 						stage = 0;
@@ -258,17 +271,72 @@ namespace
 				}
 			}
 		}
-		else if (warp > Cfg::kMmaWarp)
+		else if (warp == Cfg::kScaleWarp)
+		{
+			/* scale i * 32 + lane of a slot belongs to token (i * 32 + lane) % TOKENS of block kb + (i * 32 + lane) / TOKENS; the factors
+			 * of the next kAhead slots are on their way while this warp waits for a buffer */
+			constexpr int kScales = kPerStage * TOKENS / 32, kAhead = 2;
+			float next_a[kAhead][kScales], next_b[kAhead][kScales];
+			auto fetch = [&](float (&va)[kScales], float (&vb)[kScales], int kb)
+			{
+#pragma unroll
+				for (int i = 0; i < kScales; i++)
+				{
+					const int t = m0 + (i * 32 + lane) % TOKENS, g = kb + (i * 32 + lane) / TOKENS;
+					const bool inside = g < last and t < p.M;
+					va[i] = inside ? p.a_scale[static_cast<long long>(t) * p.blocks + g] : 0.0f;
+					vb[i] = inside ? p.b_scale[static_cast<long long>(n_block) * p.blocks + g] : 0.0f;
+				}
+			};
+#pragma unroll
+			for (int u = 0; u < kAhead; u++)
+				fetch(next_a[u], next_b[u], first + u * kPerStage);
+			int stage = 0, buffer = 0;
+			uint32_t buffer_phase = 0;
+			bool ok = true;
+			for (int kb0 = first; kb0 < last and ok; kb0 += kAhead * kPerStage)
+			{
+#pragma unroll
+				for (int u = 0; u < kAhead; u++)
+				{
+					const int kb = kb0 + u * kPerStage;
+					if (kb >= last)
+						break;
+					ok = __all_sync(0xFFFFFFFFu, lane != 0 or umma::mbar_wait(&drained_bar[buffer], buffer_phase ^ 1u, abort_ptr));
+					if (not ok)
+					{
+						if (lane == 0)
+							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
+						break;
+					}
+#pragma unroll
+					for (int i = 0; i < kScales; i++)
+						scale_s[buffer][i * 32 + lane] = next_a[u][i] * next_b[u][i];
+					__syncwarp();
+					if (lane == 0)
+						umma::mbar_arrive(&done_bar[stage]);
+					fetch(next_a[u], next_b[u], kb + kAhead * kPerStage);
+					if (++stage == kStages)
+						stage = 0;
+					if (++buffer == Cfg::kBuffers)
+					{
+						buffer = 0;
+						buffer_phase ^= 1u;
+					}
+				}
+			}
+		}
+		else if (warp > Cfg::kScaleWarp)
 		{
 			if (LOADERS or lane == 0)
 			{
-				const int thread = threadIdx.x - Cfg::kPromoteThreads - 32;
+				const int thread = threadIdx.x - Cfg::kPromoteThreads - 64;
 				int stage = 0;
 				uint32_t phase = 0;
 				for (int kb = first; kb < last; kb += kPerStage)
 				{
 					const int count = min(kPerStage, last - kb);
-					if (not umma::mbar_wait(&drained_bar[stage], phase ^ 1u, abort_ptr))
+					if (not umma::mbar_wait(&done_bar[stage], phase ^ 1u, abort_ptr))
 					{
 						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorStageWait);
 						break;
@@ -319,86 +387,58 @@ namespace
 		{
 			/* promotion: lane = row n0 + row of B, one accumulator per token of the warp's share */
 			constexpr int kTokens = Cfg::kTokensPerWarp;
-			constexpr int kScales = kPerStage * kTokens / 32; /* scales of a slot per lane */
-			static_assert(kPerStage * kTokens % 32 == 0 and kTokens % 16 == 0, "whole warps of scales, whole loads of TMEM");
 			const int row = warp % 4 * 32 + lane;
 			const int token0 = warp / 4 * kTokens;
 			float acc[kTokens];
 #pragma unroll
 			for (int t = 0; t < kTokens; t++)
 				acc[t] = 0.0f;
-			/* the scales of the next two slots, as they come from memory: multiplied only when they are needed */
-			float next_a[2][kScales], next_b[2][kScales];
-			auto fetch = [&](float (&va)[kScales], float (&vb)[kScales], int kb)
-			{
-#pragma unroll
-				for (int i = 0; i < kScales; i++)
-				{
-					const int t = m0 + token0 + (i * 32 + lane) % kTokens, g = kb + (i * 32 + lane) / kTokens;
-					const bool inside = g < last and t < p.M;
-					va[i] = inside ? p.a_scale[static_cast<long long>(t) * p.blocks + g] : 0.0f;
-					vb[i] = inside ? p.b_scale[static_cast<long long>(n_block) * p.blocks + g] : 0.0f;
-				}
-			};
-			fetch(next_a[0], next_b[0], first);
-			fetch(next_a[1], next_b[1], first + kPerStage);
 			const uint32_t lanes = tmem_base + (static_cast<uint32_t>(warp % 4 * 32) << 16) + static_cast<uint32_t>(token0);
-			int stage = 0;
+			int stage = 0, buffer = 0;
 			uint32_t phase = 0;
 			bool ok = true;
-			for (int kb0 = first; kb0 < last and ok; kb0 += 2 * kPerStage)
+			for (int kb = first; kb < last; kb += kPerStage)
 			{
-#pragma unroll
-				for (int u = 0; u < 2; u++)
+				ok = __all_sync(0xFFFFFFFFu, lane != 0 or umma::mbar_wait(&done_bar[stage], phase, abort_ptr));
+				if (not ok)
 				{
-					const int kb = kb0 + u * kPerStage;
-					if (kb >= last)
+					if (lane == 0)
+						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
+					break;
+				}
+				umma::tcgen05_fence_after();
+#pragma unroll
+				for (int j = 0; j < kPerStage; j++)
+				{
+					if (kb + j >= last)
 						break;
-					__syncwarp(); /* the scales of the slot before have been read */
 #pragma unroll
-					for (int i = 0; i < kScales; i++)
-						scale_s[warp][i * 32 + lane] = next_a[u][i] * next_b[u][i];
-					__syncwarp();
-					fetch(next_a[u], next_b[u], kb + 2 * kPerStage);
-					ok = __all_sync(0xFFFFFFFFu, lane != 0 or umma::mbar_wait(&done_bar[stage], phase, abort_ptr));
-					if (not ok)
+					for (int t0 = 0; t0 < kTokens; t0 += 16)
 					{
-						if (lane == 0)
-							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
-						break;
-					}
-					umma::tcgen05_fence_after();
+						uint32_t r[16];
+						umma::tmem_load_32x16(lanes + static_cast<uint32_t>((buffer * kPerStage + j) * TOKENS + t0), r);
+						umma::tmem_load_wait(r);
 #pragma unroll
-					for (int j = 0; j < kPerStage; j++)
-					{
-						if (kb + j >= last)
-							break;
-#pragma unroll
-						for (int t0 = 0; t0 < kTokens; t0 += 16)
+						for (int t = 0; t < 16; t += 4)
 						{
-							uint32_t r[16];
-							umma::tmem_load_32x16(lanes + static_cast<uint32_t>((stage * kPerStage + j) * TOKENS + t0), r);
-							umma::tmem_load_wait(r);
-#pragma unroll
-							for (int t = 0; t < 16; t += 4)
-							{
-								const float4 s = *reinterpret_cast<const float4*>(&scale_s[warp][j * kTokens + t0 + t]);
-								acc[t0 + t] = fmaf(__uint_as_float(r[t]), s.x, acc[t0 + t]);
-								acc[t0 + t + 1] = fmaf(__uint_as_float(r[t + 1]), s.y, acc[t0 + t + 1]);
-								acc[t0 + t + 2] = fmaf(__uint_as_float(r[t + 2]), s.z, acc[t0 + t + 2]);
-								acc[t0 + t + 3] = fmaf(__uint_as_float(r[t + 3]), s.w, acc[t0 + t + 3]);
-							}
+							const float4 s = *reinterpret_cast<const float4*>(&scale_s[buffer][j * TOKENS + token0 + t0 + t]);
+							acc[t0 + t] = fmaf(__uint_as_float(r[t]), s.x, acc[t0 + t]);
+							acc[t0 + t + 1] = fmaf(__uint_as_float(r[t + 1]), s.y, acc[t0 + t + 1]);
+							acc[t0 + t + 2] = fmaf(__uint_as_float(r[t + 2]), s.z, acc[t0 + t + 2]);
+							acc[t0 + t + 3] = fmaf(__uint_as_float(r[t + 3]), s.w, acc[t0 + t + 3]);
 						}
 					}
-					umma::tcgen05_fence_before();
-					__syncwarp();
-					if (lane == 0)
-						umma::mbar_arrive(&drained_bar[stage]);
-					if (++stage == kStages)
-					{
-						stage = 0;
-						phase ^= 1u;
-					}
+				}
+				umma::tcgen05_fence_before();
+				__syncwarp();
+				if (lane == 0)
+					umma::mbar_arrive(&drained_bar[buffer]);
+				if (++buffer == Cfg::kBuffers)
+					buffer = 0;
+				if (++stage == kStages)
+				{
+					stage = 0;
+					phase ^= 1u;
 				}
 			}
 			/* Every MMA of this CTA has run (this warp waited for the last one), and each of them had waited for its copies: the
@@ -424,20 +464,23 @@ namespace
 			for (int i = rank * Cfg::kPromoteThreads + threadIdx.x; i < tokens * 32; i += splits * Cfg::kPromoteThreads)
 			{
 				const int n = i % 32 * 4;
-				float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-				for (int q = 0; q < splits; q++)
+				/* every CTA's part is requested before the first is added */
+				float4 part[kMaxSplits];
+				if (splits > 1)
 				{
-					float4 v;
-					if (splits > 1)
-						asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-								: "r"(umma::map_to_cta(partial + static_cast<uint32_t>(i) * 16u, static_cast<uint32_t>(q))) : "memory");
-					else
-						v = reinterpret_cast<const float4*>(smem)[i];
-					sum.x += v.x;
-					sum.y += v.y;
-					sum.z += v.z;
-					sum.w += v.w;
+#pragma unroll
+					for (int q = 0; q < kMaxSplits; q++)
+						if (q < splits)
+							asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(part[q].x), "=f"(part[q].y), "=f"(part[q].z), "=f"(part[q].w)
+									: "r"(umma::map_to_cta(partial + static_cast<uint32_t>(i) * 16u, static_cast<uint32_t>(q))));
 				}
+				else
+					part[0] = reinterpret_cast<const float4*>(smem)[i];
+				float4 sum = part[0];
+#pragma unroll
+				for (int q = 1; q < kMaxSplits; q++)
+					if (q < splits)
+						sum = make_float4(sum.x + part[q].x, sum.y + part[q].y, sum.z + part[q].z, sum.w + part[q].w);
 				if (n0 + n < p.N)
 					finish_four(p, static_cast<long long>(m0 + i / 32) * p.N + n0 + n, sum, min(4, p.N - n0 - n));
 			}
