@@ -111,7 +111,8 @@ namespace
 	 * full[s] (copy -> MMA) and done[s] (MMA and scales -> promotion, and back to the copies: the slot may be filled again) go round
 	 * over the slots of shared memory, drained[b] (promotion -> MMA and scales) over the accumulators in TMEM.  Each block of K has
 	 * an accumulator of its own, because its scales are applied outside the tensor core: acc[t] += scale[t] * part[t] in float32
-	 * registers, lane = row of B.  Two blocks share a slot, so that every role waits once per eight MMAs.  A warp of its own loads
+	 * registers, lane = row of B.  Two blocks share a slot, so that every role waits once per eight MMAs, and two threads issue the
+	 * MMAs of every other slot each (one takes 1150 cycles per slot, twice what the MMAs need).  A warp of its own loads
 	 * the scales, slots ahead of their use, and hands them to all promotion warps through shared memory.
 	 *
 	 * LOADERS: four warps fill the slots with plain loads instead of the TMA copies, for row pitches or addresses that are no
@@ -135,9 +136,9 @@ namespace
 			static constexpr int kPromoteWarps = TOKENS > 32 ? 8 : 4;
 			static constexpr int kPromoteThreads = kPromoteWarps * 32;
 			static constexpr int kTokensPerWarp = TOKENS / (kPromoteWarps / 4);
-			static constexpr int kMmaWarp = kPromoteWarps, kScaleWarp = kPromoteWarps + 1;
+			static constexpr int kMmaWarp = kPromoteWarps, kScaleWarp = kPromoteWarps + 2; /* two issuers */
 			static constexpr int kLoaderThreads = LOADERS ? 128 : 32;
-			static constexpr int kThreads = kPromoteThreads + 64 + kLoaderThreads;
+			static constexpr int kThreads = kPromoteThreads + 96 + kLoaderThreads;
 	};
 
 	/* 16 bytes from any address, zero past the first `valid`; only bytes inside [low, high) are touched */
@@ -229,15 +230,16 @@ namespace
 		chain_release();
 		chain_wait();
 
-		if (warp == Cfg::kMmaWarp)
+		if (warp == Cfg::kMmaWarp or warp == Cfg::kMmaWarp + 1)
 		{
 			if (lane == 0)
 			{
 				constexpr uint32_t idesc = umma::make_instr_desc(umma::kAccumF32, umma::kFormatE4M3, umma::kFormatE4M3, false, false, 128, TOKENS);
 				const uint64_t desc0 = umma::make_smem_desc(umma::smem_u32(smem), 16, 1024, umma::kSwizzle128B);
-				int stage = 0, buffer = 0;
+				static_assert(kStages >= 2 and Cfg::kBuffers >= 2, "two slots further wraps round at most once");
+				int stage = warp - Cfg::kMmaWarp, buffer = stage;
 				uint32_t phase = 0, buffer_phase = 0;
-				for (int kb = first; kb < last; kb += kPerStage)
+				for (int kb = first + stage * kPerStage; kb < last; kb += 2 * kPerStage)
 				{
 					if (not umma::mbar_wait(&drained_bar[buffer], buffer_phase ^ 1u, abort_ptr))
 					{
@@ -258,14 +260,16 @@ namespace
 							umma::mma_f8_k4(tmem_base + static_cast<uint32_t>((buffer * kPerStage + j) * TOKENS), desc, desc + kBlockBytes / 16, idesc, false);
 						}
 					umma::mma_commit(&done_bar[stage]);
-					if (++buffer == Cfg::kBuffers)
+					buffer += 2;
+					if (buffer >= Cfg::kBuffers)
 					{
-						buffer = 0;
+						buffer -= Cfg::kBuffers;
 						buffer_phase ^= 1u;
 					}
-					if (++stage == kStages)
+					stage += 2;
+					if (stage >= kStages)
 					{
-						stage = 0;
+						stage -= kStages;
 						phase ^= 1u;
 					}
 				}
@@ -330,7 +334,7 @@ namespace
 		{
 			if (LOADERS or lane == 0)
 			{
-				const int thread = threadIdx.x - Cfg::kPromoteThreads - 64;
+				const int thread = threadIdx.x - Cfg::kPromoteThreads - 96;
 				int stage = 0;
 				uint32_t phase = 0;
 				for (int kb = first; kb < last; kb += kPerStage)
@@ -407,32 +411,45 @@ namespace
 					break;
 				}
 				umma::tcgen05_fence_after();
+				/* The slot's accumulators of this warp, block after block, 32 columns per load and at most two loads at once; the
+				 * buffer, with its scales, is handed back at the end. */
+				constexpr int kLoads = kPerStage * kTokens / 32, kAtOnce = kLoads < 2 ? kLoads : 2;
 #pragma unroll
-				for (int j = 0; j < kPerStage; j++)
+				for (int l0 = 0; l0 < kLoads; l0 += kAtOnce)
 				{
-					if (kb + j >= last)
-						break;
+					uint32_t r[kAtOnce][32];
 #pragma unroll
-					for (int t0 = 0; t0 < kTokens; t0 += 16)
+					for (int l = 0; l < kAtOnce; l++)
 					{
-						uint32_t r[16];
-						umma::tmem_load_32x16(lanes + static_cast<uint32_t>((buffer * kPerStage + j) * TOKENS + t0), r);
-						umma::tmem_load_wait(r);
+						const int f = (l0 + l) * 32, column = f / kTokens * TOKENS + f % kTokens;
+						umma::tmem_load_32x32(lanes + static_cast<uint32_t>(buffer * kPerStage * TOKENS + column), r[l]);
+					}
 #pragma unroll
-						for (int t = 0; t < 16; t += 4)
+					for (int l = 0; l < kAtOnce; l++)
+						umma::tmem_load_wait(r[l]);
+#pragma unroll
+					for (int l = 0; l < kAtOnce; l++)
+					{
+						const int f = (l0 + l) * 32;
+						const float *scale = &scale_s[buffer][f / kTokens * TOKENS + token0 + f % kTokens];
+#pragma unroll
+						for (int e = 0; e < 32; e += 4)
 						{
-							const float4 s = *reinterpret_cast<const float4*>(&scale_s[buffer][j * TOKENS + token0 + t0 + t]);
-							acc[t0 + t] = fmaf(__uint_as_float(r[t]), s.x, acc[t0 + t]);
-							acc[t0 + t + 1] = fmaf(__uint_as_float(r[t + 1]), s.y, acc[t0 + t + 1]);
-							acc[t0 + t + 2] = fmaf(__uint_as_float(r[t + 2]), s.z, acc[t0 + t + 2]);
-							acc[t0 + t + 3] = fmaf(__uint_as_float(r[t + 3]), s.w, acc[t0 + t + 3]);
+							if (kb + (f + e) / kTokens >= last)
+								break; /* the slot's second block does not exist */
+							const float4 s = *reinterpret_cast<const float4*>(scale + e);
+							const int t = (f + e) % kTokens;
+							acc[t] = fmaf(__uint_as_float(r[l][e]), s.x, acc[t]);
+							acc[t + 1] = fmaf(__uint_as_float(r[l][e + 1]), s.y, acc[t + 1]);
+							acc[t + 2] = fmaf(__uint_as_float(r[l][e + 2]), s.z, acc[t + 2]);
+							acc[t + 3] = fmaf(__uint_as_float(r[l][e + 3]), s.w, acc[t + 3]);
 						}
 					}
 				}
 				umma::tcgen05_fence_before();
 				__syncwarp();
 				if (lane == 0)
-					umma::mbar_arrive(&drained_bar[buffer]);
+					umma::mbar_arrive(&drained_bar[buffer]); /* this warp has read the accumulators and the scales */
 				if (++buffer == Cfg::kBuffers)
 					buffer = 0;
 				if (++stage == kStages)
