@@ -481,6 +481,8 @@ namespace
 			for (int i = rank * Cfg::kPromoteThreads + threadIdx.x; i < tokens * 32; i += splits * Cfg::kPromoteThreads)
 			{
 				const int n = i % 32 * 4;
+				if (n0 + n >= p.N)
+					continue; /* before its loads: none may be on the way when the cluster's CTAs leave */
 				/* every CTA's part is requested before the first is added */
 				float4 part[kMaxSplits];
 				if (splits > 1)
@@ -498,8 +500,7 @@ namespace
 				for (int q = 1; q < kMaxSplits; q++)
 					if (q < splits)
 						sum = make_float4(sum.x + part[q].x, sum.y + part[q].y, sum.z + part[q].z, sum.w + part[q].w);
-				if (n0 + n < p.N)
-					finish_four(p, static_cast<long long>(m0 + i / 32) * p.N + n0 + n, sum, min(4, p.N - n0 - n));
+				finish_four(p, static_cast<long long>(m0 + i / 32) * p.N + n0 + n, sum, min(4, p.N - n0 - n));
 			}
 		}
 		umma::tcgen05_fence_before();
