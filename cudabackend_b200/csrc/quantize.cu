@@ -39,18 +39,66 @@ namespace
 	{
 		return __float_as_uint(x) & 0x7FFFFFFFu;
 	}
-	__device__ __forceinline__ uint32_t max_over_half_warp(uint32_t v)
-	{
-#pragma unroll
-		for (int i = kLanes / 2; i > 0; i /= 2)
-			v = max(v, __shfl_xor_sync(kFullWarp, v, i));
-		return v;
-	}
 	/* the clamped maximum as a float; NaN passes (its bit pattern is above that of 2^-100) */
 	__device__ __forceinline__ float clamped_amax(uint32_t bits)
 	{
 		return __uint_as_float(max(bits, __float_as_uint(kSmallestAmax)));
 	}
+	/* The maxima of up to four blocks, each held in parts by the 16 lanes of a half-warp, reduced together: every exchange halves
+	 * what a lane is responsible for (five shuffles for four blocks instead of sixteen), so that lane l ends with block
+	 * item_of(l)'s maximum and the two divisions are done once for all of them. */
+	template<int ITEMS>
+	struct BlockFactors
+	{
+			static_assert(ITEMS >= 1 and ITEMS <= 4, "blocks of one half-warp");
+			float factor; /* 448 / max(amax, 2^-100) of block item_of(lane) */
+			float scale;  /* max(amax, 2^-100) / 448 */
+
+			__device__ __forceinline__ explicit BlockFactors(const uint32_t (&bits)[ITEMS])
+			{
+				const int l = threadIdx.x % kLanes;
+				uint32_t own = bits[0];
+				if constexpr (ITEMS == 1)
+					own = max(own, __shfl_xor_sync(kFullWarp, own, 8));
+				else if constexpr (ITEMS == 2)
+				{
+					const uint32_t other = (l & 8) ? bits[0] : bits[1];
+					own = (l & 8) ? bits[1] : bits[0];
+					own = max(own, __shfl_xor_sync(kFullWarp, other, 8));
+				}
+				else
+				{
+					const uint32_t last = ITEMS == 4 ? bits[ITEMS - 1] : 0u;
+					const uint32_t other0 = (l & 8) ? bits[0] : bits[2], other1 = (l & 8) ? bits[1] : last;
+					uint32_t own0 = (l & 8) ? bits[2] : bits[0], own1 = (l & 8) ? last : bits[1];
+					own0 = max(own0, __shfl_xor_sync(kFullWarp, other0, 8));
+					own1 = max(own1, __shfl_xor_sync(kFullWarp, other1, 8));
+					const uint32_t other = (l & 4) ? own0 : own1;
+					own = (l & 4) ? own1 : own0;
+					own = max(own, __shfl_xor_sync(kFullWarp, other, 4));
+				}
+				if constexpr (ITEMS <= 2)
+					own = max(own, __shfl_xor_sync(kFullWarp, own, 4));
+				own = max(own, __shfl_xor_sync(kFullWarp, own, 2));
+				own = max(own, __shfl_xor_sync(kFullWarp, own, 1));
+				const float amax = clamped_amax(own);
+				factor = kLargestE4m3 / amax;
+				scale = amax / kLargestE4m3;
+			}
+			/* the block whose values a lane holds, and the lane that stores them */
+			__device__ __forceinline__ static int item_of(int l)
+			{
+				return ITEMS == 1 ? 0 : ITEMS == 2 ? l / 8 : l / 4;
+			}
+			__device__ __forceinline__ static bool stores(int l)
+			{
+				return l % (ITEMS == 1 ? 16 : ITEMS == 2 ? 8 : 4) == 0 and item_of(l) < ITEMS;
+			}
+			__device__ __forceinline__ float factor_of(int item) const
+			{
+				return __shfl_sync(kFullWarp, factor, item * (ITEMS == 2 ? 8 : 4), kLanes);
+			}
+	};
 	__device__ __forceinline__ uint32_t four_codes(const float *x, float r)
 	{
 		const uint32_t low = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[0], r), __fmul_rn(x[1], r)), __NV_SATFINITE, __NV_E4M3);
@@ -206,18 +254,6 @@ namespace
 			bits = __vmaxu2(bits, pairs[i] & 0x7FFF7FFFu);
 		return bits;
 	}
-	/* over the lanes that differ in the bits below `lanes`, as a clamped float */
-	template<typename T, int LANES>
-	__device__ __forceinline__ uint32_t raw_max_over_lanes(uint32_t bits)
-	{
-#pragma unroll
-		for (int i = LANES / 2; i > 0; i /= 2)
-		{
-			const uint32_t other = __shfl_xor_sync(kFullWarp, bits, i);
-			bits = sizeof(T) == 4 ? max(bits, other) : __vmaxu2(bits, other);
-		}
-		return bits;
-	}
 	template<typename T>
 	__device__ __forceinline__ uint32_t float_bits(uint32_t bits) /* of the larger half */
 	{
@@ -289,14 +325,17 @@ namespace
 				load_eight<VEC>(v[i], x + offset[i], column[i], l, columns);
 				a.advance(next_rows, next_blocks, blocks);
 			}
+			uint32_t bits[kAtOnce];
 #pragma unroll
 			for (int i = 0; i < kAtOnce; i++)
-			{
-				const float amax = clamped_amax(float_bits<T>(raw_max_over_lanes<T, kLanes>(raw_max(v[i], 0u))));
-				store_codes<VEC>(y + offset[i], v[i], kLargestE4m3 / amax, column[i], l, columns);
-				if (l == 0 and column[i] < columns)
-					scales[b + i * kHalfWarps] = amax / kLargestE4m3;
-			}
+				bits[i] = float_bits<T>(raw_max(v[i], 0u));
+			const BlockFactors<kAtOnce> f(bits);
+#pragma unroll
+			for (int i = 0; i < kAtOnce; i++)
+				store_codes<VEC>(y + offset[i], v[i], f.factor_of(i), column[i], l, columns);
+			const long long own = b + f.item_of(l) * kHalfWarps;
+			if (f.stores(l) and own < total)
+				scales[own] = f.scale;
 			b += static_cast<long long>(gridDim.x) * (kHalfWarps * kAtOnce);
 			at.advance(strideRows, strideBlocks, blocks);
 		}
@@ -330,7 +369,7 @@ namespace
 #pragma unroll
 			for (int p = 0; p < kPasses; p++)
 				bits = raw_max(v[p], bits);
-			bits = float_bits<T>(raw_max_over_lanes<T, 32>(bits));
+			bits = __reduce_max_sync(kFullWarp, float_bits<T>(bits));
 			if (threadIdx.x % 32 == 0)
 				warp_max[turn][threadIdx.x / 32] = bits;
 			__syncthreads(); /* two sets of slots: the next turn's writes cannot meet this turn's reads */
@@ -380,20 +419,16 @@ namespace
 					v[i] += other[i];
 			}
 		};
-		auto finish = [&](float (&v)[kPerLane], const float (&g)[kPerLane], int b, float rstd)
+		auto scaled = [&](float (&v)[kPerLane], const float (&g)[kPerLane], int b, float rstd)
 		{
-			const int column = b * kScaleBlock;
 			if (h != nullptr)
-				store_eight<VEC>(h + offset, v, column, l, limit);
+				store_eight<VEC>(h + offset, v, b * kScaleBlock, l, limit);
 			uint32_t bits = 0;
 #pragma unroll
 			for (int i = 0; i < kPerLane; i++)
 				v[i] = __fmul_rn(__fmul_rn(v[i], rstd), g[i]);
 			largest_magnitude(v, bits);
-			const float amax = clamped_amax(max_over_half_warp(bits));
-			store_codes<VEC>(y + offset, v, kLargestE4m3 / amax, column, l, limit);
-			if (l == 0 and b < blocks and inside)
-				scales[row * blocks + b] = amax / kLargestE4m3;
+			return bits;
 		};
 		auto square_sum = [](const float (&v)[kPerLane], float sum)
 		{
@@ -458,13 +493,21 @@ namespace
 		const float rstd = 1.0f / sqrtf(sum / static_cast<float>(columns) + epsilon);
 		if constexpr (ITEMS > 0)
 		{
+			uint32_t bits[kHeld];
 #pragma unroll
 			for (int i = 0; i < kHeld; i++)
 			{
 				if constexpr (not kGammaFirst)
 					load_eight<VEC>(g, gamma, (half + i * halves) * kScaleBlock, l, limit);
-				finish(v[i], g, half + i * halves, rstd);
+				bits[i] = scaled(v[i], g, half + i * halves, rstd);
 			}
+			const BlockFactors<kHeld> f(bits);
+#pragma unroll
+			for (int i = 0; i < kHeld; i++)
+				store_codes<VEC>(y + offset, v[i], f.factor_of(i), (half + i * halves) * kScaleBlock, l, limit);
+			const int own = half + f.item_of(l) * halves;
+			if (f.stores(l) and own < blocks and inside)
+				scales[row * blocks + own] = f.scale;
 		}
 		else
 		{
@@ -473,7 +516,11 @@ namespace
 			{
 				load_sum(v[0], b * kScaleBlock);
 				load_eight<VEC>(g, gamma, b * kScaleBlock, l, limit);
-				finish(v[0], g, b, rstd);
+				const uint32_t bits[1] = { scaled(v[0], g, b, rstd) };
+				const BlockFactors<1> f(bits);
+				store_codes<VEC>(y + offset, v[0], f.factor, b * kScaleBlock, l, limit);
+				if (l == 0 and b < blocks and inside)
+					scales[row * blocks + b] = f.scale;
 			}
 		}
 	}
