@@ -393,8 +393,8 @@ namespace
 	/* ---- norm + quantise ------------------------------------------------------------------------------------------------
 	 * `halves` half-warps (a power of two) share a row; number i of them owns the blocks i, i + halves, ... .  ITEMS > 0: at most
 	 * ITEMS blocks each, kept in registers between the sum of squares and the codes.  ITEMS = 0: rows of any length, read twice. */
-	template<typename T, int ITEMS, bool VEC>
-	__global__ void __launch_bounds__(1024) kernel_rms_norm_quantize(const T *x, const T *z, T *h, const float *__restrict__ gamma, uint8_t *__restrict__ y,
+	template<typename T, int ITEMS, bool VEC, int THREADS>
+	__global__ void __launch_bounds__(THREADS) kernel_rms_norm_quantize(const T *x, const T *z, T *h, const float *__restrict__ gamma, uint8_t *__restrict__ y,
 			float *__restrict__ scales, long long rows, int columns, int blocks, int halves, float epsilon)
 	{
 		__shared__ float warp_sum[32];
@@ -568,6 +568,13 @@ namespace
 			int columns;
 			float epsilon;
 	};
+	template<typename T, bool VEC, int THREADS>
+	auto norm_kernel(int items)
+	{
+		return items <= 1 ? kernel_rms_norm_quantize<T, 1, VEC, THREADS> : items <= 2 ? kernel_rms_norm_quantize<T, 2, VEC, THREADS> :
+				items <= 3 ? kernel_rms_norm_quantize<T, 3, VEC, THREADS> : items <= 4 ? kernel_rms_norm_quantize<T, 4, VEC, THREADS> :
+				kernel_rms_norm_quantize<T, 0, VEC, THREADS>;
+	}
 	template<typename T, bool VEC>
 	avStatus_t launch_norm(ContextObject &ctx, const NormArgs &a)
 	{
@@ -587,8 +594,7 @@ namespace
 		const long long grid = (a.rows + rows_per_block - 1) / rows_per_block;
 		if (grid > 0x7FFFFFFFll)
 			return AVOCADO_STATUS_NOT_SUPPORTED;
-		auto kernel = per_half <= 1 ? kernel_rms_norm_quantize<T, 1, VEC> : per_half <= 2 ? kernel_rms_norm_quantize<T, 2, VEC> :
-				per_half <= 3 ? kernel_rms_norm_quantize<T, 3, VEC> : per_half <= 4 ? kernel_rms_norm_quantize<T, 4, VEC> : kernel_rms_norm_quantize<T, 0, VEC>;
+		auto kernel = threads <= kThreads ? norm_kernel<T, VEC, kThreads>(per_half) : norm_kernel<T, VEC, 1024>(per_half);
 		const cudaError_t launched = launch_chained(kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, ctx.getStream(),
 				reinterpret_cast<const T*>(a.x.ptr), reinterpret_cast<const T*>(a.z.ptr), reinterpret_cast<T*>(a.h.ptr), reinterpret_cast<const float*>(a.gamma.ptr),
 				a.y.ptr, reinterpret_cast<float*>(a.scales.ptr), a.rows, a.columns, blocks, halves, a.epsilon);
