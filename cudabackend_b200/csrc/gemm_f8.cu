@@ -105,8 +105,8 @@ namespace
 	 * that a handful of tokens does not waste 128-row tiles; the result is transposed on the way out.
 	 *
 	 * Bound: the bytes of B.  One tile of 128 rows of B per CTA leaves most SMs without work at the usual sizes, so the blocks of
-	 * K are split over the CTAs of a cluster; their partial sums meet in distributed shared memory and are added in the order
-	 * of the ranks (no scratch memory, no atomics, the same bits every time).
+	 * K are split over the CTAs of a cluster.  Each CTA finishes a share of the tokens and adds everybody's partial sums for these in
+	 * the order of the ranks: no scratch memory, no atomics, the same bits every time.
 	 *
 	 * full[s] (copy -> MMA) and done[s] (MMA and scales -> promotion, and back to the copies: the slot may be filled again) go round
 	 * over the slots of shared memory, drained[b] (promotion -> MMA and scales) over the accumulators in TMEM.  Each block of K has
@@ -129,7 +129,11 @@ namespace
 			/* Two CTAs of different clusters never share an SM: each could wait for the TMEM of the other's neighbour. */
 			static constexpr int kSmemBytes = kStages * kStageBytes + 1024;
 			static_assert(kSmemBytes > 116 * 1024 and kSmemBytes <= 228 * 1024, "one CTA per SM");
-			static_assert(TOKENS * 512 <= kStages * kStageBytes, "the partial sums reuse the slots");
+			/* How partial sums meet: where they are few, every CTA sends its own, float by float, to the CTA that finishes the token;
+			 * where they are many, they stay where they are and are read from there.  Graph of 1 x 4096 x 4096: 4.9 us sent, 5.6
+			 * read; 128 x 4096 x 4096: 11.2 us sent, 11.3 copied in bulk, 10.0 read. */
+			static constexpr bool kSendSums = TOKENS <= 32;
+			static_assert((TOKENS + kMaxSplits) * 512 <= kStages * kStageBytes, "the partial sums reuse the slots");
 			static constexpr int kWantedColumns = kBuffers * kPerStage * TOKENS;
 			static constexpr int kTmemColumns = kWantedColumns <= 128 ? 128 : kWantedColumns <= 256 ? 256 : 512;
 			/* promotion warps: four for the 128 lanes of TMEM, twice that where each would hold more than 32 tokens */
@@ -186,6 +190,7 @@ namespace
 		__shared__ __align__(8) uint64_t full_bar[kStages];
 		__shared__ __align__(8) uint64_t done_bar[kStages];
 		__shared__ __align__(8) uint64_t drained_bar[Cfg::kBuffers];
+		__shared__ __align__(8) uint64_t sums_bar; /* the other CTAs' partial sums for this CTA's tokens have arrived */
 		__shared__ uint32_t tmem_base_slot;
 		__shared__ int abort_flag;
 		__shared__ __align__(16) float scale_s[Cfg::kBuffers][kPerStage * TOKENS];
@@ -199,6 +204,9 @@ namespace
 		const int n0 = n_block * 128;
 		const int first = min(p.blocks, rank * blocksPerSplit);
 		const int last = min(p.blocks, first + blocksPerSplit);
+		const int tokens = min(TOKENS, p.M - m0);
+		const int share = (tokens + splits - 1) / splits; /* CTA r finishes tokens r * share .. */
+		const int own_tokens = max(0, min(share, tokens - rank * share));
 
 		if (threadIdx.x == 0)
 		{
@@ -210,7 +218,9 @@ namespace
 			}
 			for (int b = 0; b < Cfg::kBuffers; b++)
 				umma::mbar_init(&drained_bar[b], Cfg::kPromoteWarps);
+			umma::mbar_init(&sums_bar, 1);
 			umma::mbar_fence_init();
+			umma::mbar_arrive_expect_tx(&sums_bar, static_cast<uint32_t>((splits - 1) * own_tokens * 512));
 			if (not LOADERS)
 			{
 				umma::prefetch_tensormap(&mapA);
@@ -387,13 +397,13 @@ namespace
 				}
 			}
 		}
-		else
+		constexpr int kTokens = Cfg::kTokensPerWarp;
+		const int row = warp % 4 * 32 + lane;
+		const int token0 = warp / 4 * kTokens;
+		float acc[kTokens];
+		if (warp < Cfg::kPromoteWarps)
 		{
 			/* promotion: lane = row n0 + row of B, one accumulator per token of the warp's share */
-			constexpr int kTokens = Cfg::kTokensPerWarp;
-			const int row = warp % 4 * 32 + lane;
-			const int token0 = warp / 4 * kTokens;
-			float acc[kTokens];
 #pragma unroll
 			for (int t = 0; t < kTokens; t++)
 				acc[t] = 0.0f;
@@ -403,7 +413,7 @@ namespace
 			bool ok = true;
 			for (int kb = first; kb < last; kb += kPerStage)
 			{
-				ok = __all_sync(0xFFFFFFFFu, lane != 0 or umma::mbar_wait(&done_bar[stage], phase, abort_ptr));
+				ok = __all_sync(0xFFFFFFFFu, umma::mbar_wait(&done_bar[stage], phase, abort_ptr));
 				if (not ok)
 				{
 					if (lane == 0)
@@ -458,55 +468,88 @@ namespace
 					phase ^= 1u;
 				}
 			}
-			/* Every MMA of this CTA has run (this warp waited for the last one), and each of them had waited for its copies: the
-			 * slots are free to take the partial sums, token after token. */
-			if (ok)
-			{
-				float *partial = reinterpret_cast<float*>(smem);
-#pragma unroll
-				for (int t = 0; t < kTokens; t++)
-					partial[(token0 + t) * 128 + row] = acc[t];
-			}
 		}
 
 		__syncthreads();
 		if (abort_flag != 0)
 			umma::drain_after_abort();
-		if (splits > 1)
-			umma::cluster_sync_all(); /* the partial sums of every CTA are written */
-		if (threadIdx.x < Cfg::kPromoteThreads and abort_flag == 0)
+		/* Every MMA of a CTA that has come here has run (its promotion warps waited for the last one), and each had waited for its
+		 * copies: its slots are free to take partial sums. */
+		if (Cfg::kSendSums and splits > 1)
+			umma::cluster_sync_all_relaxed();
+		/* rows of 128 floats; sent: part of CTA q for token i of this CTA's share at row q * share + i; read: own part for token i of
+		 * the tile at row i */
+		float *sums = reinterpret_cast<float*>(smem);
+		const uint32_t bar = umma::smem_u32(&sums_bar);
+		if (warp < Cfg::kPromoteWarps)
 		{
-			const int tokens = min(TOKENS, p.M - m0);
-			const uint32_t partial = umma::smem_u32(smem);
-			for (int i = rank * Cfg::kPromoteThreads + threadIdx.x; i < tokens * 32; i += splits * Cfg::kPromoteThreads)
+			int owner = token0 / share, place = token0 - owner * share;
+#pragma unroll
+			for (int t = 0; t < kTokens; t++)
+			{
+				if (token0 + t < tokens)
+				{
+					float *to = sums + (Cfg::kSendSums ? rank * share + place : token0 + t) * 128 + row;
+					if (not Cfg::kSendSums or owner == rank)
+						*to = acc[t];
+					else
+						umma::store_async_cluster(umma::map_to_cta(umma::smem_u32(to), static_cast<uint32_t>(owner)), acc[t],
+								umma::map_to_cta(bar, static_cast<uint32_t>(owner)));
+				}
+				if (++place == share)
+				{
+					place = 0;
+					owner++;
+				}
+			}
+		}
+		umma::tcgen05_fence_before();
+		__syncthreads(); /* this CTA's own part is written */
+		if (not Cfg::kSendSums and splits > 1)
+			umma::cluster_sync_all(); /* and so is everybody's */
+		if (threadIdx.x < Cfg::kPromoteThreads and own_tokens > 0)
+		{
+			bool arrived = true;
+			if (Cfg::kSendSums)
+			{
+				/* the CTA may leave only when everything that is sent to it has arrived, whether or not a wait ran out before */
+				volatile int ignored = 0;
+				arrived = umma::mbar_wait(&sums_bar, 0, &ignored) and umma::mbar_try_wait_cluster(&sums_bar, 0);
+				if (not arrived)
+					umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
+			}
+			for (int i = threadIdx.x; arrived and i < own_tokens * 32; i += Cfg::kPromoteThreads)
 			{
 				const int n = i % 32 * 4;
 				if (n0 + n >= p.N)
 					continue; /* before its loads: none may be on the way when the cluster's CTAs leave */
-				/* every CTA's part is requested before the first is added */
 				float4 part[kMaxSplits];
-				if (splits > 1)
-				{
 #pragma unroll
-					for (int q = 0; q < kMaxSplits; q++)
-						if (q < splits)
+				for (int q = 0; q < kMaxSplits; q++)
+					if (q < splits)
+					{
+						if (Cfg::kSendSums)
+							part[q] = reinterpret_cast<const float4*>(sums)[q * share * 32 + i];
+						else if (splits > 1)
 							asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(part[q].x), "=f"(part[q].y), "=f"(part[q].z), "=f"(part[q].w)
-									: "r"(umma::map_to_cta(partial + static_cast<uint32_t>(i) * 16u, static_cast<uint32_t>(q))));
-				}
-				else
-					part[0] = reinterpret_cast<const float4*>(smem)[i];
+									: "r"(umma::map_to_cta(umma::smem_u32(sums) + static_cast<uint32_t>(rank * share * 32 + i) * 16u, static_cast<uint32_t>(q))));
+						else
+							part[q] = reinterpret_cast<const float4*>(sums)[i];
+					}
 				float4 sum = part[0];
 #pragma unroll
 				for (int q = 1; q < kMaxSplits; q++)
 					if (q < splits)
 						sum = make_float4(sum.x + part[q].x, sum.y + part[q].y, sum.z + part[q].z, sum.w + part[q].w);
-				finish_four(p, static_cast<long long>(m0 + i / 32) * p.N + n0 + n, sum, min(4, p.N - n0 - n));
+				finish_four(p, static_cast<long long>(m0 + rank * share + i / 32) * p.N + n0 + n, sum, min(4, p.N - n0 - n));
 			}
 		}
-		umma::tcgen05_fence_before();
-		__syncthreads();
-		if (splits > 1)
-			umma::cluster_sync_all(); /* nobody leaves while its partial sums may still be read */
+		if (not Cfg::kSendSums)
+		{
+			__syncthreads();
+			if (splits > 1)
+				umma::cluster_sync_all_relaxed(); /* nobody leaves while its sums may still be read; what was read has been used */
+		}
 		if (warp == Cfg::kMmaWarp)
 		{
 			umma::tcgen05_fence_after();

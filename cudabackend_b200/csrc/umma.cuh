@@ -321,6 +321,25 @@ namespace umma
 	{
 		asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 	}
+	/* the same without publishing memory writes (a release at cluster scope costs 1000 cycles and more): enough where a CTA only
+	 * says that it has reached a point, and for barriers made visible by mbar_fence_init */
+	__device__ __forceinline__ void cluster_sync_all_relaxed()
+	{
+		asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+	}
+	/* whether the phase is complete, ordering what other CTAs of the cluster wrote before it in front of what follows */
+	__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity)
+	{
+		uint32_t done = 0;
+		asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+				: "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+		return done != 0;
+	}
+	/* writes one float into a CTA's shared memory and counts its four bytes on an mbarrier of that CTA */
+	__device__ __forceinline__ void store_async_cluster(uint32_t clusterAddr, float value, uint32_t clusterBar)
+	{
+		asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(clusterAddr), "f"(value), "r"(clusterBar) : "memory");
+	}
 	__device__ __forceinline__ void mbar_arrive_cluster(uint32_t clusterAddr)
 	{
 		asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(clusterAddr) : "memory");
