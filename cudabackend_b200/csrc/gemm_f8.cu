@@ -115,8 +115,8 @@ namespace
 	 * MMAs of every other slot each (one takes 1150 cycles per slot, twice what the MMAs need).  A warp of its own loads
 	 * the scales, slots ahead of their use, and hands them to all promotion warps through shared memory.
 	 *
-	 * LOADERS: four warps fill the slots with plain loads instead of the TMA copies, for row pitches or addresses that are no
-	 * multiple of 16 bytes.
+	 * LOADERS: eight warps fill the slots with plain loads instead of the TMA copies, for row pitches or addresses that are no
+	 * multiple of 16 bytes; at most 64 tokens, because of their registers.
 	 */
 	template<int TOKENS, bool LOADERS>
 	struct SplitConfig
@@ -141,41 +141,80 @@ namespace
 			static constexpr int kPromoteThreads = kPromoteWarps * 32;
 			static constexpr int kTokensPerWarp = TOKENS / (kPromoteWarps / 4);
 			static constexpr int kMmaWarp = kPromoteWarps, kScaleWarp = kPromoteWarps + 2; /* two issuers */
-			static constexpr int kLoaderThreads = LOADERS ? 128 : 32;
+			static constexpr int kLoaderWarps = LOADERS ? 8 : 1, kLoaderThreads = kLoaderWarps * 32;
 			static constexpr int kThreads = kPromoteThreads + 96 + kLoaderThreads;
 	};
 
-	/* 16 bytes from any address, zero past the first `valid`; only bytes inside [low, high) are touched */
-	__device__ __forceinline__ uint4 load_unaligned(const uint8_t *ptr, int valid, const uint8_t *low, const uint8_t *high)
+	/* Plain loads into a slot: one row of at most 256 bytes (its two blocks) per warp and turn.  Rows start at any address, so lane
+	 * l loads the aligned words l and l + 32 that cover it and shifts neighbours together.  Word l of a block's row lies in piece
+	 * (l / 4) ^ (row % 8), the 128-byte swizzle that the descriptors name. */
+	__device__ __forceinline__ uint32_t* slot_word(uint8_t *slot, int row, int lane)
 	{
-		uint32_t w[5];
-		const int offset = static_cast<int>(reinterpret_cast<uintptr_t>(ptr) & 3);
-		const uint8_t *base = ptr - offset;
-#pragma unroll
-		for (int i = 0; i < 5; i++)
+		return reinterpret_cast<uint32_t*>(slot + row * 128 + ((lane / 4) ^ (row & 7)) * 16 + lane % 4 * 4);
+	}
+	/* The aligned words reach up to three bytes outside the row: rows within four bytes of an end of the tensor go byte by byte. */
+	__device__ __noinline__ void store_edge_row(uint8_t *slot, int row, int pairBytes, const uint8_t *from, int valid, int lane)
+	{
+		for (int block = 0; block < 2; block++)
 		{
-			const uint8_t *at = base + 4 * i;
-			w[i] = 0;
-			if (4 * i < offset + valid)
+			uint32_t word = 0;
+			for (int i = 0; i < 4; i++)
+				if (block * 128 + 4 * lane + i < valid)
+					word |= static_cast<uint32_t>(from[block * 128 + 4 * lane + i]) << (8 * i);
+			slot_word(slot, row, lane)[block * pairBytes / 4] = word;
+		}
+	}
+	/* ROWS rows of an operand, kLoaderWarps apart: all requested before the first is stored.  `rows`: how many of the tensor's rows
+	 * there are from the first one on; start: its offset in the tensor of `total` bytes. */
+	template<int ROWS, int STEP>
+	__device__ __forceinline__ void load_rows(uint8_t *slot, int row0, int pairBytes, const uint8_t *tensor, long long start, long long total, int rows, int pitch,
+			int columns, int lane)
+	{
+		uint32_t low[ROWS], high[ROWS], next[ROWS];
+		bool any_edge = false;
+		const long long step = static_cast<long long>(STEP) * pitch;
+		auto end_of = [&](int i, long long at)
+		{
+			const bool edge = at < 4 or at + columns + 4 > total;
+			return i * STEP < rows and not edge ? static_cast<int>(reinterpret_cast<uintptr_t>(tensor + at) & 3) + columns : 0;
+		};
+#pragma unroll
+		for (int i = 0; i < ROWS; i++)
+		{
+			const long long at = start + i * step;
+			const int end = end_of(i, at);
+			any_edge = any_edge or (end == 0 and i * STEP < rows);
+			const uint32_t *words = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(tensor + at) & ~static_cast<uintptr_t>(3));
+			low[i] = 4 * lane < end ? words[lane] : 0u;
+			high[i] = 4 * lane + 128 < end ? words[lane + 32] : 0u;
+			next[i] = (lane == 31 and 256 < end) ? words[64] : 0u;
+		}
+#pragma unroll
+		for (int i = 0; i < ROWS; i++)
+		{
+			const int shift = 8 * static_cast<int>(reinterpret_cast<uintptr_t>(tensor + start + i * step) & 3);
+			uint32_t after_low = __shfl_down_sync(0xFFFFFFFFu, low[i], 1), after_high = __shfl_down_sync(0xFFFFFFFFu, high[i], 1);
+			const uint32_t high_first = __shfl_sync(0xFFFFFFFFu, high[i], 0);
+			if (lane == 31)
 			{
-				if (at >= low and at + 4 <= high)
-					w[i] = *reinterpret_cast<const uint32_t*>(at);
-				else
-					for (int j = 0; j < 4; j++)
-						if (at + j >= low and at + j < high)
-							w[i] |= static_cast<uint32_t>(at[j]) << (8 * j);
+				after_low = high_first;
+				after_high = next[i];
 			}
+			/* bytes past the last column are zeros: of this lane's word at byte c, columns - c are kept */
+			const int keep_low = min(max(columns - 4 * lane, 0), 4), keep_high = min(max(columns - 4 * lane - 128, 0), 4);
+			const uint32_t mask_low = keep_low == 4 ? 0xFFFFFFFFu : (1u << (8 * keep_low)) - 1u, mask_high = keep_high == 4 ? 0xFFFFFFFFu : (1u << (8 * keep_high)) - 1u;
+			uint32_t *to = slot_word(slot, row0 + i * STEP, lane);
+			to[0] = __funnelshift_r(low[i], after_low, shift) & mask_low;
+			to[pairBytes / 4] = __funnelshift_r(high[i], after_high, shift) & mask_high;
 		}
-		uint32_t r[4];
-#pragma unroll
-		for (int i = 0; i < 4; i++)
-		{
-			r[i] = __funnelshift_r(w[i], w[i + 1], 8 * offset);
-			const int left = valid - 4 * i;
-			if (left < 4)
-				r[i] = left <= 0 ? 0u : r[i] & ((1u << (8 * left)) - 1u);
-		}
-		return make_uint4(r[0], r[1], r[2], r[3]);
+		if (any_edge)
+#pragma unroll 1
+			for (int i = 0; i < ROWS; i++)
+			{
+				const long long at = start + i * step;
+				if (i * STEP < rows and end_of(i, at) == 0)
+					store_edge_row(slot, row0 + i * STEP, pairBytes, tensor + at, columns, lane);
+			}
 	}
 
 	template<int TOKENS, bool LOADERS>
@@ -358,25 +397,16 @@ namespace
 					uint8_t *slot = smem + stage * Cfg::kStageBytes;
 					if constexpr (LOADERS)
 					{
-						/* piece i of a row lies at piece i ^ (row % 8): the 128-byte swizzle that the descriptors name */
-						for (int j = 0; j < count; j++)
-						{
-							const int k = (kb + j) * kScaleBlock + thread % 8 * 16;
-							const int valid = max(0, min(16, p.K - k));
-#pragma unroll 4
-							for (int row = thread / 8; row < 128 + TOKENS; row += Cfg::kLoaderThreads / 8)
-							{
-								const bool weights = row < 128;
-								const int r = weights ? row : row - 128;
-								const long long global = weights ? n0 + static_cast<long long>(r) : m0 + static_cast<long long>(r);
-								const long long rows = weights ? p.N : p.M;
-								const uint8_t *base = weights ? p.b : p.a;
-								uint4 v = make_uint4(0, 0, 0, 0);
-								if (global < rows and valid > 0)
-									v = load_unaligned(base + global * p.K + k, valid, base, base + rows * p.K);
-								*reinterpret_cast<uint4*>(slot + j * Cfg::kPairBytes + (weights ? 0 : kBlockBytes) + r * 128 + ((thread % 8) ^ (r & 7)) * 16) = v;
-							}
-						}
+						static_assert(kPerStage == 2, "a row of the slot is two blocks");
+						constexpr int kStep = Cfg::kLoaderWarps;
+						const int k = kb * kScaleBlock, loader = thread / 32;
+						const int columns = min(count * kScaleBlock, p.K - k);
+#pragma unroll 1
+						for (int part = 0; part < 128; part += 8 * kStep)
+							load_rows<8, kStep>(slot, part + loader, Cfg::kPairBytes, p.b, (static_cast<long long>(n0) + part + loader) * p.K + k,
+									static_cast<long long>(p.N) * p.K, p.N - n0 - part - loader, p.K, columns, lane);
+						load_rows<TOKENS / kStep, kStep>(slot + kBlockBytes, loader, Cfg::kPairBytes, p.a, (static_cast<long long>(m0) + loader) * p.K + k,
+								static_cast<long long>(p.M) * p.K, p.M - m0 - loader, p.K, columns, lane);
 						umma::fence_proxy_async_smem();
 						umma::mbar_arrive(&full_bar[stage]);
 					}
@@ -423,7 +453,7 @@ namespace
 				umma::tcgen05_fence_after();
 				/* The slot's accumulators of this warp, block after block, 32 columns per load and at most two loads at once; the
 				 * buffer, with its scales, is handed back at the end. */
-				constexpr int kLoads = kPerStage * kTokens / 32, kAtOnce = kLoads < 2 ? kLoads : 2;
+				constexpr int kLoads = kPerStage * kTokens / 32, kAtOnce = LOADERS or kLoads < 2 ? 1 : 2;
 #pragma unroll
 				for (int l0 = 0; l0 < kLoads; l0 += kAtOnce)
 				{
@@ -1046,9 +1076,9 @@ namespace
 			return launch_split<16, LOADERS>(ctx, p);
 		if (p.M <= 32)
 			return launch_split<32, LOADERS>(ctx, p);
-		if (p.M <= 64)
+		if (LOADERS or p.M <= 64)
 			return launch_split<64, LOADERS>(ctx, p);
-		return launch_split<128, LOADERS>(ctx, p);
+		return launch_split<128, false>(ctx, p);
 	}
 
 	template<typename T, bool ADD>
