@@ -4,6 +4,14 @@
  * src/gemm.cpp:42-57).
  *
  *   C[m, n] = alpha * sum_g aScale[m, g] * bScale[n / 128, g] * P_g[m, n] + beta * C[m, n],   P_g = sum over block g of A * B
+ *
+ * P_g comes from tcgen05.mma kind::f8f6f4 (products exact, float32 accumulators in TMEM).  The scales are arbitrary float32
+ * numbers, which the tensor core cannot apply, so every block of 128 gets an accumulator of its own and a "promotion" in
+ * float32 registers, acc += scale * P_g: one read of the accumulator and one fused multiply-add per result and block, on the CUDA
+ * cores, beside the MMAs of the next block.  Measured against float64 the result is off by 6e-8 (float32 C, 333 x 2056 x 1616).
+ *
+ * Two kernels: kernel_gemm_f8_split (few rows of A, unaligned rows, few tiles; K split over a cluster) and kernel_gemm_f8_pair (256 x
+ * 256 tiles on CTA pairs).  The choice is in launch(), with both sides measured.
  */
 #include <Avocado/cuda_backend_ext.h>
 
@@ -104,7 +112,9 @@ namespace
 	 * Few rows of A ("tokens"), and any row pitch: 128 rows of B are the M side of the MMA and TOKENS rows of A its N side, so
 	 * that a handful of tokens does not waste 128-row tiles; the result is transposed on the way out.
 	 *
-	 * Bound: the bytes of B.  One tile of 128 rows of B per CTA leaves most SMs without work at the usual sizes, so the blocks of
+	 * Bound: the bytes of B in principle; at these sizes the set-up (1000 cycles), the first copy (1200) and the end (1500) of a CTA
+	 * that lives 8000 cycles.  Measured in a graph: 1 x 4096 x 4096 4.8 us (3.5 TB/s), 13 x 8192 x 4096 9.1 us (3.7 TB/s), 1 x 8192 x
+	 * 8192 13.1 us (5.1 TB/s), 128 x 4096 x 4096 9.8 us, 333 x 2056 x 1616 10.1 us.  One tile of 128 rows of B per CTA leaves most SMs without work at the usual sizes, so the blocks of
 	 * K are split over the CTAs of a cluster.  Each CTA finishes a share of the tokens and adds everybody's partial sums for these in
 	 * the order of the ranks: no scratch memory, no atomics, the same bits every time.
 	 *
@@ -116,7 +126,8 @@ namespace
 	 * the scales, slots ahead of their use, and hands them to all promotion warps through shared memory.
 	 *
 	 * LOADERS: eight warps fill the slots with plain loads instead of the TMA copies, for row pitches or addresses that are no
-	 * multiple of 16 bytes; at most 64 tokens, because of their registers.
+	 * multiple of 16 bytes; at most 64 tokens, because of their registers.  Bound by the latency of the loads that those registers
+	 * hold (24 KB per SM): 1 x 4096 x 4095 13 us, 500 x 3000 x 1001 33 us, 4096 x 4096 x 4095 740 us.
 	 */
 	template<int TOKENS, bool LOADERS>
 	struct SplitConfig
@@ -592,11 +603,20 @@ namespace
 	 * the rows of B, holds 128 x 256 accumulators in float32 registers (128 per thread of eight warps) and the two newest blocks
 	 * of K in TMEM.
 	 *
-	 * Why 256 x 256: per block of K a CTA pulls 32 KB from L2 for 558 cycles of MMAs (four of N = 256, 139.5 cycles each),
-	 * 59 bytes per cycle; 128 x 128 tiles on single CTAs pull 32 KB for 344 cycles.  The promotion acc += scale * part reads
-	 * 128 x 256 floats of TMEM per block of K and issues 256 packed fused multiply-adds per scheduler, which fits beside the MMAs.
+	 * Why 256 x 256: per block of K a CTA pulls 32 KB from L2 for 524 cycles of MMAs (four of N = 256, 131 cycles each), 62
+	 * bytes per cycle, about what L2 delivers; 128 x 128 tiles on single CTAs pull the same 32 KB for 280 cycles.  The promotion
+	 * reads 128 x 256 floats of TMEM per block of K and issues 256 fused multiply-adds per scheduler (packed pairs were slower:
+	 * 690 cycles of promotion per block against 500).
+	 *
+	 * What bounds it: the round trip of an accumulator (MMAs 524 cycles, commit to wake-up 200, promotion 500, arrival to the next
+	 * MMA 250) over the two that fit in TMEM: 890 cycles per block where the MMAs alone take 524, and, over long runs, the
+	 * power limit (8192^3: 517 us for tens of milliseconds, 600 us at the clocks of seconds).  Measured and not kept: accumulators of
+	 * 128 columns (twice the MMAs to issue, 1020 cycles per block), sixteen promotion warps (621 us against 511), loads of 32
+	 * columns (the same).
 	 * Why two issuing threads: a block of K costs its issuer two waits, four MMAs and two commits, about 680 cycles, more
 	 * than the MMAs take; even and odd blocks have an issuer (and an accumulator) each.
+	 *
+	 * Measured (bfloat16 C): 8192^3 517 us, 2130 TFLOP/s; 4096 x 8192 x 4096 134 us; 50176 x 256 x 2304 38 us (2.65 waves of tiles).
 	 *
 	 *   full[s]        first CTA only: its producer posts the bytes of both CTAs' copies
 	 *   empty[s]       both CTAs: the commit after a slot's MMAs
@@ -1012,8 +1032,8 @@ namespace
 		return umma::make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 	}
 
-	/* CTAs per tile: the number that ends first, where a CTA's time is its blocks of K plus about kOverhead blocks of set-up, first
-	 * copy and reduction, and one CTA runs per SM. */
+	/* CTAs per tile: the number that ends first, where a CTA's time is its blocks of K (about 350 cycles each) plus that of
+	 * kOverhead blocks for set-up, first copy and reduction, and one CTA runs per SM. */
 	int choose_splits(long long tiles, int blocks, int sms)
 	{
 		constexpr int kOverhead = 6;
@@ -1135,6 +1155,9 @@ namespace
 			const cudaError_t launched = launch_chained(kernel_scale_c, grid, dim3(256), 0, ctx.getStream(), p);
 			return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
 		}
+		/* Few tiles leave most pairs idle, and 256-row tiles waste what few rows of A do not fill.  bfloat16 C, us, pairs / split:
+		 * 256 x 4096 x 4096 (16 tiles) 20.4 / 14.6, 1024^3 (16) 8.5 / 8.6, 333 x 2056 x 1616 (18) 11.2 / 10.1, 512 x 4096 x 4096 (32)
+		 * 20.9 / 21.2, 4096 x 512 x 4096 (32) 21.1 / 27.1, 2048^3 (64) 13.9 / 25.6. */
 		const bool tma = p.K % 16 == 0 and (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0;
 		if (tma and p.M > 128 and static_cast<long long>((p.M + 255) / 256) * ((p.N + 255) / 256) >= 32)
 			return launch_pair(ctx, p);
