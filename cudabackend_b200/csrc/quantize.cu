@@ -14,7 +14,7 @@
  *
  * Bound: HBM.  Measured (of 6566 GB/s copied): 4096 x 8192 bfloat16 to 1 x 128 blocks 20.8 us (102 MB, 0.74; a plain copy of that
  * size takes 20 us), 8192 x 8192 to 128 x 128 blocks 34.9 us (201 MB, 0.88), norm of 8192 x 8192 with residual 80 us (470 MB, 0.89),
- * norm of 50176 x 264 float16 15.3 us (40 MB, 0.39: instructions, 240 per row; a block's work does not shrink with its 8 of 128
+ * norm of 50176 x 264 float16 14.3 us (40 MB, 0.43: instructions, over 200 per row; a block's work does not shrink with its 8 of 128
  * columns).
  */
 #include <Avocado/cuda_backend_ext.h>
@@ -235,12 +235,32 @@ namespace
 			}
 		}
 	}
-	__device__ __forceinline__ float largest_magnitude(const float (&v)[kPerLane], uint32_t &bits)
+	/* the largest magnitude as an integer; max.NaN keeps a NaN, whose positive pattern is above every number's */
+	template<bool PACKED>
+	__device__ __forceinline__ uint32_t largest_magnitude(const float (&v)[kPerLane])
 	{
+		if constexpr (not PACKED)
+		{
+			uint32_t bits = 0;
 #pragma unroll
-		for (int i = 0; i < kPerLane; i++)
-			bits = max(bits, magnitude_bits(v[i]));
-		return __uint_as_float(bits);
+			for (int i = 0; i < kPerLane; i++)
+				bits = max(bits, magnitude_bits(v[i]));
+			return bits;
+		}
+		float largest = fabsf(v[0]);
+#pragma unroll
+		for (int i = 1; i < kPerLane; i++)
+			asm("max.NaN.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(v[i])));
+		return __float_as_uint(largest) & 0x7FFFFFFFu;
+	}
+	/* two products, each rounded like a product of its own, in one instruction */
+	__device__ __forceinline__ void multiply_pair(float &x0, float &x1, float y0, float y1)
+	{
+		asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1));
+	}
+	__device__ __forceinline__ void square_pair(float &sum0, float &sum1, float x0, float x1)
+	{
+		asm("{\n\t.reg .b64 s, x;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 x, {%2, %3};\n\tfma.rn.f32x2 s, x, x, s;\n\tmov.b64 {%0, %1}, s;\n\t}" : "+f"(sum0), "+f"(sum1) : "f"(x0), "f"(x1));
 	}
 
 	/* The largest magnitude of raw elements as an integer; two 16-bit patterns are compared at once. */
@@ -404,6 +424,9 @@ namespace
 	__global__ void __launch_bounds__(THREADS) kernel_rms_norm_quantize(const T *x, const T *z, T *h, const float *__restrict__ gamma, uint8_t *__restrict__ y,
 			float *__restrict__ scales, long long rows, int columns, int blocks, int halves, float epsilon)
 	{
+		/* Pairs in one instruction where instructions are what bounds (short rows: 50176 x 264 float16 15.3 -> 14.3 us); with four
+		 * blocks per half-warp their registers cost a resident thread block (8192 x 8192: 80 -> 89 us). */
+		constexpr bool kPacked = ITEMS != 4;
 		__shared__ float warp_sum[32];
 		chain_release();
 		chain_wait();
@@ -430,25 +453,39 @@ namespace
 		{
 			if (h != nullptr)
 				store_eight<VEC>(h + offset, v, b * kScaleBlock, l, limit);
-			uint32_t bits = 0;
+			if constexpr (kPacked)
+			{
 #pragma unroll
-			for (int i = 0; i < kPerLane; i++)
-				v[i] = __fmul_rn(__fmul_rn(v[i], rstd), g[i]);
-			largest_magnitude(v, bits);
-			return bits;
+				for (int i = 0; i < kPerLane; i += 2)
+				{
+					multiply_pair(v[i], v[i + 1], rstd, rstd);
+					multiply_pair(v[i], v[i + 1], g[i], g[i + 1]);
+				}
+			}
+			else
+			{
+#pragma unroll
+				for (int i = 0; i < kPerLane; i++)
+					v[i] = __fmul_rn(__fmul_rn(v[i], rstd), g[i]);
+			}
+			return largest_magnitude<kPacked>(v);
 		};
-		auto square_sum = [](const float (&v)[kPerLane], float sum)
+		float sum = 0.0f, odd_sum = 0.0f;
+		auto add_squares = [&](const float (&v)[kPerLane])
 		{
 #pragma unroll
 			for (int i = 0; i < kPerLane; i++)
-				sum = fmaf(v[i], v[i], sum);
-			return sum;
+			{
+				if constexpr (not kPacked)
+					sum = fmaf(v[i], v[i], sum);
+				else if (i % 2 == 0)
+					square_pair(sum, odd_sum, v[i], v[i + 1]);
+			}
 		};
 
 		constexpr int kHeld = ITEMS > 0 ? ITEMS : 1;
 		constexpr bool kGammaFirst = ITEMS == 1; /* a row per block: gamma's latency is hidden behind the row's, not added to it */
 		float v[kHeld][kPerLane], g[kPerLane];
-		float sum = 0.0f;
 		if constexpr (ITEMS > 0)
 		{
 			{
@@ -471,17 +508,19 @@ namespace
 				load_eight<VEC>(g, gamma, half * kScaleBlock, l, limit);
 #pragma unroll
 			for (int i = 0; i < kHeld; i++)
-				sum = square_sum(v[i], sum);
+				add_squares(v[i]);
 		}
 		else
 		{
 			for (int b = half; b < blocks; b += halves)
 			{
 				load_sum(v[0], b * kScaleBlock);
-				sum = square_sum(v[0], sum);
+				add_squares(v[0]);
 			}
 			__syncwarp();
 		}
+		if constexpr (kPacked)
+			sum += odd_sum;
 #pragma unroll
 		for (int i = kLanes / 2; i > 0; i /= 2)
 			sum += __shfl_xor_sync(kFullWarp, sum, i);

@@ -251,3 +251,29 @@ def test_offsets_past_32_bits(ctx, n, k):
         got = c.to_host(ctx, np.empty((keep, n), dtype=np.uint16), first * n * 2)
         ctx.synchronize()
         assert np.all(np.abs(api.bfloat16_bits_to_float(got) - ref) <= bs.gemm_error_bound(ref, size, k, "bfloat16"))
+
+
+def test_the_other_calls_refuse_the_type(ctx):
+    """entry points that compute with elements know nothing of e4m3; cudaIm2Row, which only moves them, is tested with the chain"""
+    dtype = api.STATUS["UNSUPPORTED_DATATYPE"]
+    a, b, c = (bs.Placed(ctx, (32, 32), "float8_e4m3") for _ in range(3))
+    args = (a.desc.handle, a.mem.handle, b.desc.handle, b.mem.handle, None, c.desc.handle, c.mem.handle)
+    assert api.call_status("cudaGemm", ctx.handle, 0, 1, None, *args) == dtype
+    a3, b3, c3 = (bs.Placed(ctx, (1, 32, 32), "float8_e4m3") for _ in range(3))
+    args = (a3.desc.handle, a3.mem.handle, b3.desc.handle, b3.mem.handle, None, c3.desc.handle, c3.mem.handle)
+    assert api.call_status("cudaGemmBatched", ctx.handle, 0, 1, None, *args) == dtype
+    f = bs.Placed(ctx, (32, 32), "float32")
+    args = (a.desc.handle, a.mem.handle, b.desc.handle, b.mem.handle, None, f.desc.handle, f.mem.handle)
+    assert api.call_status("cudaGemm", ctx.handle, 0, 1, None, *args) == dtype
+    assert api.call_status("cudaActivationForward", ctx.handle, 3, None, a.desc.handle, a.mem.handle, None, b.desc.handle, b.mem.handle) == dtype
+    bias = bs.Placed(ctx, (32,), "float32")
+    assert api.call_status("cudaAddBias", ctx.handle, None, None, a.desc.handle, a.mem.handle, bias.desc.handle, bias.mem.handle, b.desc.handle, b.mem.handle,
+                           None, None, None, api.INVALID, 0) == dtype
+    conv = api.ConvolutionDescriptor(api.CONVOLUTION_MODE, (-1, -1))
+    x, w, y = bs.Placed(ctx, (1, 8, 8, 16), "float8_e4m3"), bs.Placed(ctx, (16, 3, 3, 16), "float8_e4m3"), bs.Placed(ctx, (1, 8, 8, 16), "float8_e4m3")
+    for entry in ("cudaConvolutionImplicitGemmForward", "cudaConvolutionWinogradFusedForward"):
+        status = api.call_status(entry, ctx.handle, conv.handle, None, x.desc.handle, x.mem.handle, w.desc.handle, w.mem.handle, api.INVALID, api.INVALID, None,
+                                 api.INVALID, api.INVALID, None, y.desc.handle, y.mem.handle, 0)
+        assert status in (dtype, api.STATUS["NOT_SUPPORTED"]), entry
+    for t in (a, b, c, c3, f, y):
+        assert np.all(t.raw().view(np.uint8) == 0x5A) and t.guards_intact()
