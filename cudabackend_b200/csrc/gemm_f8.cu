@@ -400,7 +400,10 @@ namespace
 				for (int kb = first; kb < last; kb += kPerStage)
 				{
 					const int count = min(kPerStage, last - kb);
-					if (not umma::mbar_wait(&done_bar[stage], phase ^ 1u, abort_ptr))
+					bool ready = umma::mbar_wait(&done_bar[stage], phase ^ 1u, abort_ptr);
+					if constexpr (LOADERS)
+						ready = __all_sync(0xFFFFFFFFu, ready); /* a warp's lanes exchange words below */
+					if (not ready)
 					{
 						umma::raise_error(abort_ptr, deviceStatus, umma::kErrorStageWait);
 						break;
