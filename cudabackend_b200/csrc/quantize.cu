@@ -617,9 +617,10 @@ namespace
 	template<typename T, bool VEC, int THREADS>
 	auto norm_kernel(int items)
 	{
+		if (items > 4) /* more than 64 half-warps of four: blocks of 1024 threads only */
+			return kernel_rms_norm_quantize<T, 0, VEC, 1024>;
 		return items <= 1 ? kernel_rms_norm_quantize<T, 1, VEC, THREADS> : items <= 2 ? kernel_rms_norm_quantize<T, 2, VEC, THREADS> :
-				items <= 3 ? kernel_rms_norm_quantize<T, 3, VEC, THREADS> : items <= 4 ? kernel_rms_norm_quantize<T, 4, VEC, THREADS> :
-				kernel_rms_norm_quantize<T, 0, VEC, THREADS>;
+				items <= 3 ? kernel_rms_norm_quantize<T, 3, VEC, THREADS> : kernel_rms_norm_quantize<T, 4, VEC, THREADS>;
 	}
 	template<typename T, bool VEC>
 	avStatus_t launch_norm(ContextObject &ctx, const NormArgs &a)
