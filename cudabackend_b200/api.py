@@ -250,6 +250,22 @@ class Graph:
             pass
 
 
+class Address(int):
+    """A device address that keeps the Memory it points into alive, so that whoever holds the address (a tensor made from it through
+    __cuda_array_interface__, say) may outlive the object that it was asked of.  Sums keep it too; Memory.destroy() frees at once."""
+
+    def __new__(cls, value, memory):
+        self = super().__new__(cls, value)
+        self.memory = memory
+        return self
+
+    def __add__(self, offset):
+        total = int(self) + offset
+        return Address(total, self.memory) if isinstance(total, int) else total
+
+    __radd__ = __add__
+
+
 class Memory:
     """avMemoryDescriptor_t: an owning device allocation (or a view of one)."""
 
@@ -271,7 +287,7 @@ class Memory:
     def pointer(self):
         p = _VP()
         call("cudaGetMemoryPointer", self.handle, ctypes.byref(p))
-        return p.value or 0
+        return Address(p.value or 0, self)
 
     def from_host(self, ctx, array, offset=0):
         array = np.ascontiguousarray(array)
