@@ -273,6 +273,7 @@ class Memory:
         self.size = int(size)
         self.device = device
         self._owned = owned
+        self._viewed = None  # the memory that this is a view of, which has to live as long
         if handle is None:
             h = _H(INVALID)
             call("cudaCreateMemoryDescriptor", ctypes.byref(h), device, self.size)
@@ -282,7 +283,9 @@ class Memory:
     def view(self, size, offset):
         h = _H(INVALID)
         call("cudaCreateMemoryView", ctypes.byref(h), self.handle, int(size), int(offset))
-        return Memory(size, self.device, handle=h.value)
+        result = Memory(size, self.device, handle=h.value)
+        result._viewed = self
+        return result
 
     def pointer(self):
         p = _VP()

@@ -17,7 +17,7 @@ def destroyed(monkeypatch):
         if name == "cudaGetMemoryPointer":
             args[1]._obj.value = 0x1000 * args[0]
         elif name == "cudaCreateMemoryView":
-            args[0]._obj.value = 100 + args[1]
+            args[0]._obj.value = 100 + args[3]
         elif name == "cudaDestroyMemoryDescriptor":
             handles.append(args[0])
 
@@ -47,6 +47,17 @@ def test_destroy_frees_whoever_holds_the_address(destroyed):
     del memory, address
     gc.collect()
     assert destroyed == [7]
+
+
+def test_a_view_keeps_the_memory_it_looks_into(destroyed):
+    view = api.Memory(64, handle=7).view(32, 8)
+    inner = view.view(8, 4)
+    del view
+    gc.collect()
+    assert destroyed == []
+    del inner
+    gc.collect()
+    assert sorted(destroyed) == [7, 104, 108]
 
 
 @pytest.mark.gpu
