@@ -133,18 +133,16 @@ def _in_hand(held):
     blocks = {k: api.DeviceTensor(tuple(v.shape), names[v.dtype]) for k, v in held.items()}
     views = {}
     for k, v in held.items():
-        views[k] = _view(blocks[k], v)
+        views[k] = _view(blocks[k].mem.pointer(), v)
         views[k].copy_(v)
     torch.cuda.synchronize()
     return {"t": views, "d": blocks, "ctx": api.Context.default(0), "api": api}
 
 
-def _view(block, like):
+def _view(pointer, like):
     class Holder:
         pass
     holder = Holder()
-    holder.block = block  # the tensor keeps its holder, and with it the memory that it looks into
-    pointer = block.mem.pointer()
     holder.__cuda_array_interface__ = {"shape": (like.numel() * like.element_size(),), "typestr": "|u1", "data": (pointer, False), "version": 3}
     return torch.as_tensor(holder, device="cuda").view(like.dtype).view(like.shape)
 
