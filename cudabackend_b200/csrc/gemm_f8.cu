@@ -654,10 +654,11 @@ namespace
 		return t;
 	}
 	/* One 32-row sub-tile of C (64 16-bit or 32 float32 columns) from registers: staged in the swizzled order of the store's tensor
-	 * map, then written by one bulk copy, or row by row where C's pitch or address rules the copy out. */
+	 * map, then written by one bulk copy, or row by row where C's pitch or address rules the copy out.  first: of a tile; the copies
+	 * of the tile before, which end with either buffer where its last columns are past N, have read both before it is overwritten. */
 	template<typename T, bool ADD>
 	__device__ __forceinline__ void store_sub_tile(const ScaledGemm &p, const CUtensorMap *mapC, uint8_t *buffer, const float *acc, int row0, int column0, int lane,
-			bool bulk)
+			bool bulk, bool first)
 	{
 		constexpr int kColumns = 128 / static_cast<int>(sizeof(T));
 		constexpr int kPerPiece = 16 / static_cast<int>(sizeof(T));
@@ -666,7 +667,12 @@ namespace
 		if (bulk)
 		{
 			if (lane == 0)
-				umma::tma_store_wait_read<1>(); /* the copy before last has read this buffer */
+			{
+				if (first)
+					umma::tma_store_wait_read<0>();
+				else
+					umma::tma_store_wait_read<1>(); /* the copy before last has read this buffer */
+			}
 			__syncwarp();
 		}
 		const T *old = reinterpret_cast<const T*>(p.c) + static_cast<long long>(row0 + lane) * p.N + column0;
@@ -734,7 +740,7 @@ namespace
 		constexpr int kColumns = 128 / static_cast<int>(sizeof(T));
 #pragma unroll
 		for (int sub = 0; sub < 128 / kColumns; sub++)
-			store_sub_tile<T, ADD>(p, mapC, buffers + (sub & 1) * kSubBytes, acc + sub * kColumns, row0, column0 + sub * kColumns, lane, bulk);
+			store_sub_tile<T, ADD>(p, mapC, buffers + (sub & 1) * kSubBytes, acc + sub * kColumns, row0, column0 + sub * kColumns, lane, bulk, sub == 0);
 	}
 
 	/* ADD: beta is not 0.  The type of C and this are template parameters because the store runs once per tile, out of a cold

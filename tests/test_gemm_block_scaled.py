@@ -277,3 +277,24 @@ def test_the_other_calls_refuse_the_type(ctx):
         assert status in (dtype, api.STATUS["NOT_SUPPORTED"]), entry
     for t in (a, b, c, c3, f, y):
         assert np.all(t.raw().view(np.uint8) == 0x5A) and t.guards_intact()
+
+
+# More tiles than CTA pairs, so that a pair stores one tile behind another, with next to no contraction in between, and last columns
+# that leave a warp with one or three sub-tiles of C (64 16-bit or 32 float32 columns): both staging buffers are the next tile's.
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("alpha,beta", [(1.0, 0.0), (-0.6, 0.7)])
+@pytest.mark.parametrize("shape", [(20000, 520, 16), (20000, 328, 128), (12000, 1032, 128)])
+def test_ragged_columns_over_many_tiles(ctx, dtype, alpha, beta, shape):
+    p = Problem(ctx, *shape, dtype)
+    p.run(alpha, beta)
+    p.check(alpha, beta)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_ragged_columns_over_many_tiles_have_the_same_bits_every_time(ctx, dtype):
+    p = Problem(ctx, 20000, 520, 16, dtype)
+    p.run()
+    first = p.c.raw().copy()
+    for _ in range(20):
+        p.run()
+        assert np.array_equal(first.view(np.uint8), p.c.raw().view(np.uint8))
