@@ -252,7 +252,10 @@ class Graph:
 
 class Address(int):
     """A device address that keeps the Memory it points into alive, so that whoever holds the address (a tensor made from it through
-    __cuda_array_interface__, say) may outlive the object that it was asked of.  Sums keep it too; Memory.destroy() frees at once."""
+    __cuda_array_interface__, say) may outlive the object that it was asked of.  Sums keep it too; Memory.destroy() frees at once.
+
+    torch (2.11 at least) never gives back its reference to the interface's "data" tuple: memory whose address stood in one lasts until
+    destroy() or the end of the process.  Where that matters, put int(address) there and let the holder refer to the memory."""
 
     def __new__(cls, value, memory):
         self = super().__new__(cls, value)
