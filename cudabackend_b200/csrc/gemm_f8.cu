@@ -373,6 +373,7 @@ namespace
 							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
 						break;
 					}
+					__syncwarp(); /* a vote orders no memory: what lane 0 has waited for is ordered before the other lanes' writes here */
 #pragma unroll
 					for (int i = 0; i < kScales; i++)
 						scale_s[buffer][i * 32 + lane] = next_a[u][i] * next_b[u][i];
@@ -977,6 +978,7 @@ namespace
 							umma::raise_error(abort_ptr, deviceStatus, umma::kErrorEpilogueWait);
 						break;
 					}
+					__syncwarp(); /* a vote orders no memory: what lane 0 has waited for is ordered before the other lanes' reads here */
 					umma::tcgen05_fence_after();
 					const uint32_t from = lanes + b * 256u;
 					uint32_t r[2][16];

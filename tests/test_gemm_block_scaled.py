@@ -298,3 +298,21 @@ def test_ragged_columns_over_many_tiles_have_the_same_bits_every_time(ctx, dtype
     for _ in range(20):
         p.run()
         assert np.array_equal(first.view(np.uint8), p.c.raw().view(np.uint8))
+
+
+@pytest.mark.parametrize("shape", [(1, 520, 8192), (32, 1032, 8192), (64, 520, 8192), (128, 264, 8192), (50, 392, 8190), (2100, 1032, 8192)])
+def test_every_block_meets_its_own_scale(ctx, shape):
+    """64 blocks of K whose scales are all different from their neighbours', over and over: integers below 2^22, so any mix-up shows"""
+    m, n, k = shape
+    p = Problem(ctx, m, n, k, "float32")
+    r = np.random.default_rng(95)
+    p.a.upload(r.integers(-2, 3, (m, k)))
+    p.b.upload(r.integers(-2, 3, (n, k)))
+    g = np.arange(bs.blocks(k))
+    p.sa.upload(np.exp2((g[None, :] + np.arange(m)[:, None]) % 4))
+    p.sb.upload(np.exp2((g[None, :] * 3 + np.arange(bs.blocks(n))[:, None]) % 3))
+    ref = p.expected()[0]
+    for _ in range(10):
+        p.c.upload(np.full((m, n), 0.5))
+        p.run()
+        assert np.array_equal(p.c.download(), ref)
