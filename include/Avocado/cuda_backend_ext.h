@@ -153,7 +153,9 @@ DLL_PUBLIC avStatus_t cudaRmsNormQuantize(avContextDescriptor_t context, const a
  *   C[m, n] = alpha * sum over g of aScale[m, g] * bScale[n / 128, g] * (sum over k in block g of A[m, k] * B[n, k]) + beta * C[m, n]
  * aDesc, bDesc: float8_e4m3; scales float32 [M, ceil(K / 128)] and [ceil(N / 128), ceil(K / 128)]; C float16, bfloat16 or
  * float32 [M, N]; extents up to 2^30; alpha and beta float.  aOp must be N and bOp T (AVOCADO_STATUS_NOT_SUPPORTED otherwise).  Sums are float32,
- * rounded once into C.  C is not read when beta is 0.  Row pitches of 16 bytes (K a multiple of 16, A and B on 16-byte
+ * rounded once into C.  C is not read when beta is 0.  The product aScale * bScale of a block is formed first, in float32: it should be 0 or a
+ * normal number (2^-126 to 2^128).  A smaller one costs up to 2^-150 * 128 * 448^2 < 2^-125 of absolute error for its block; a larger
+ * one is infinite, and so is what it adds, or NaN where the block's sum is 0.  Row pitches of 16 bytes (K a multiple of 16, A and B on 16-byte
  * boundaries) are copied by the tensor memory accelerator; other pitches are correct and slower. */
 DLL_PUBLIC avStatus_t cudaGemmBlockScaled(avContextDescriptor_t context, avGemmOperation_t aOp, avGemmOperation_t bOp, const void *alpha,
 		const avTensorDescriptor_t aDesc, const avMemoryDescriptor_t aMem, const avTensorDescriptor_t aScaleDesc, const avMemoryDescriptor_t aScaleMem,

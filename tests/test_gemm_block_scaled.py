@@ -316,3 +316,76 @@ def test_every_block_meets_its_own_scale(ctx, shape):
         p.c.upload(np.full((m, n), 0.5))
         p.run()
         assert np.array_equal(p.c.download(), ref)
+
+
+# one of every kernel and number of tokens: few rows, unaligned rows, CTA pairs
+EVERY_KERNEL = [(9, 392, 512), (30, 392, 512), (64, 392, 512), (128, 392, 512), (50, 392, 510), (2100, 1032, 512)]
+
+
+@pytest.mark.parametrize("shape", EVERY_KERNEL)
+def test_scales_up_to_the_ends_of_their_products(ctx, shape):
+    """Products of scales from 2^-126 to 2^127.  Codes are multiples of 2^-9 up to 7 * 2^-9, so every partial sum is an integer below
+    2^15 times 2^-18, and a sum of them is exact unless it lies below the normal numbers, where each of its roundings (blocks, shares of
+    K, alpha) costs 2^-150.  Zero rows stay zero however large their scale is."""
+    m, n, k = shape
+    p = Problem(ctx, m, n, k, "float32")
+    r = np.random.default_rng(96)
+    a = r.integers(-7, 8, (m, k)) * 2.0 ** -9
+    a[4::5] = 0.0
+    p.a.upload(a)
+    p.b.upload(r.integers(-7, 8, (n, k)) * 2.0 ** -9)
+    rows, columns = np.array([0.0, -66.0, 63.0, 20.0]), np.array([64.0, -60.0, 0.0, -1.0])
+    p.sa.upload(np.exp2(np.repeat(rows[r.integers(0, 4, m)][:, None], bs.blocks(k), 1)))
+    p.sb.upload(np.exp2(np.repeat(columns[np.arange(bs.blocks(n)) % 4][:, None], bs.blocks(k), 1)))
+    p.run()
+    ref, _ = p.expected()
+    got = p.c.download()
+    assert np.all(np.abs(got - ref) <= (bs.blocks(k) + 8 + 1) * 2.0 ** -150 * (np.abs(ref) < 2.0 ** -126))
+
+
+@pytest.mark.parametrize("shape", EVERY_KERNEL)
+def test_scales_past_the_ends_of_their_products(ctx, shape):
+    """a product below the normal numbers is off by 2^-150, times partial sums of up to 128 * 448^2; one past them is infinite"""
+    m, n, k = shape
+    p = Problem(ctx, m, n, k, "float32")
+    sa, sb = np.exp2(np.full(p.sa.shape, -70.0)) * 1.1, np.exp2(np.full(p.sb.shape, -66.0)) * 1.3
+    p.sa.upload(sa)
+    p.sb.upload(sb)
+    p.run()
+    ref, size = p.expected()
+    limit = bs.blocks(k) * 2.0 ** -150 * 128 * 448 ** 2
+    assert np.all(np.abs(p.c.download() - ref) <= limit + bs.gemm_error_bound(ref, size, k, "float32"))
+    a = np.ones((m, k))
+    a[1] = 0.0
+    p.a.upload(a)
+    p.b.upload(np.ones((n, k)))
+    p.sa.upload(np.full(p.sa.shape, 2.0 ** 64))
+    p.sb.upload(np.full(p.sb.shape, 2.0 ** 64))
+    p.run()
+    got = p.c.download()
+    assert np.all(np.isnan(got[1])) and np.all(np.isposinf(np.delete(got, 1, 0)))
+
+
+@pytest.mark.parametrize("shape", EVERY_KERNEL)
+def test_zero_scales_and_infinite_ones(ctx, shape):
+    """zero times anything finite is zero, zero times infinity NaN, whatever stands beside it"""
+    m, n, k = shape
+    p = Problem(ctx, m, n, k, "float32")
+    p.a.upload(np.ones((m, k)))
+    p.b.upload(np.ones((n, k)))
+    sa, sb = np.full(p.sa.shape, 2.0 ** -9), np.full(p.sb.shape, 2.0 ** -9)
+    sa[1], sa[2], sa[3], sb[1] = 0.0, np.inf, 2.0 ** -130, 2.0 ** 100
+    sa[5] = 2.0 ** -110  # with 2^-9: a normal product
+    p.sa.upload(sa)
+    p.sb.upload(sb)
+    p.run()
+    got = p.c.download()
+    ref = k * np.repeat(sa[:, :1], n, 1) * np.repeat(sb[:, 0], 128)[None, :n]
+    assert np.array_equal(got, ref)
+    sb[0] = 0.0
+    p.sb.upload(sb)
+    p.run()
+    got = p.c.download()
+    assert np.all(np.isnan(got[2, :128])) and np.all(np.isposinf(got[2, 128:]))
+    keep = np.arange(m) != 2
+    assert np.all(got[keep, :128] == 0.0) and np.array_equal(got[keep, 128:], ref[keep, 128:])
