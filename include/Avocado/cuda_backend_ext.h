@@ -144,7 +144,9 @@ DLL_PUBLIC avStatus_t cudaQuantizeBlocks(avContextDescriptor_t context, const av
  * x, z, h: float16, bfloat16 or float32, all of xDesc's type and shape, rows of at most 2^20 elements; gamma: float32 [C].  z is
  * optional (AVOCADO_INVALID_DESCRIPTOR: h = x); h is rounded once into hMem when that is given, and may be stored over x or
  * over z (the same memory, not a part of it).  Arithmetic is float32 and y is quantised without having been rounded before;
- * squares overflow where |h| exceeds 1.8e19, as in any float32 norm.  epsilon must be positive and finite as a float32. */
+ * so is the sum of squares, which should stay below 2^128: a finite row that reaches it (from a root-mean-square of 1.8e19 / sqrt(C) on)
+ * counts as infinitely long, its y is 0 (zero codes, the scale of 2^-100) and its h as ever.  Squares below 2^-126 lose bits, which
+ * shows where C * epsilon is as small.  epsilon must be positive and finite as a float32. */
 DLL_PUBLIC avStatus_t cudaRmsNormQuantize(avContextDescriptor_t context, const avTensorDescriptor_t xDesc, const avMemoryDescriptor_t xMem,
 		const avMemoryDescriptor_t zMem, avMemoryDescriptor_t hMem, const avTensorDescriptor_t gammaDesc, const avMemoryDescriptor_t gammaMem, double epsilon,
 		const avTensorDescriptor_t yDesc, avMemoryDescriptor_t yMem, const avTensorDescriptor_t scaleDesc, avMemoryDescriptor_t scaleMem);

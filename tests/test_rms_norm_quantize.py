@@ -175,3 +175,24 @@ def test_offsets_past_32_bits(ctx):
         spread = o.spread_scales(got_s, 32, c)
         assert np.array_equal(api.bfloat16_bits_to_float(got_h), h64)  # x + x is a bfloat16 number
         assert np.all(np.abs(api.float8_bits_to_float(got_y) * spread - y64) <= bs.code_error_bound(y64, spread, norm_bound(c) + 2 * bs.U32))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("columns", [1, 136, 264, 520, 8192, 33000])
+def test_sums_of_squares_up_to_float32s_end_and_past_it(ctx, dtype, columns):
+    """rows of +-2^e whose sum of squares is the last one below 2^128, and rows whose sum passes it: these give zeros, and their h"""
+    e = int(np.floor((127.99 - np.log2(columns)) / 2))
+    r = np.random.default_rng(87)
+    shape = (6, columns)
+    x0 = np.where(r.random(shape) < 0.5, -1.0, 1.0) * np.exp2([[e], [e + 1], [0.0], [e], [e + 1], [60.0 + 60.0]])
+    x, h = bs.Placed(ctx, shape, dtype, values=x0), bs.Placed(ctx, shape, dtype)
+    gamma = bs.Placed(ctx, (columns,), "float32", values=1 + 0.2 * r.normal(0, 1, columns))
+    y, s = bs.Placed(ctx, shape, "float8_e4m3"), bs.Placed(ctx, (6, bs.blocks(columns)), "float32")
+    bs.rms_norm_quantize(ctx, x, None, h, gamma, EPSILON, y, s)
+    assert np.array_equal(h.download(), x0) and y.guards_intact() and s.guards_intact()
+    q, scales = y.download(), s.download()
+    past, keep = [1, 4, 5], [0, 2, 3]
+    assert np.all(q[past] == 0.0) and np.all(scales[past] == np.float32(2.0 ** -100) / np.float32(448))
+    _, y64 = o.rms_norm(x0[keep], None, gamma.values, EPSILON)
+    spread = o.spread_scales(scales[keep], 3, columns)
+    assert np.all(np.abs(q[keep] * spread - y64) <= bs.code_error_bound(y64, spread, norm_bound(columns) + 2 * bs.U32))
