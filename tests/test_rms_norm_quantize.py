@@ -196,3 +196,54 @@ def test_sums_of_squares_up_to_float32s_end_and_past_it(ctx, dtype, columns):
     _, y64 = o.rms_norm(x0[keep], None, gamma.values, EPSILON)
     spread = o.spread_scales(scales[keep], 3, columns)
     assert np.all(np.abs(q[keep] * spread - y64) <= bs.code_error_bound(y64, spread, norm_bound(columns) + 2 * bs.U32))
+
+
+# Rows enough to fill the machine with a half-warp (or two) per row of two to four blocks, so that different rows share a warp's
+# shuffles and the joint maxima; the last thread block has rows past the end.  333 and 131 columns take the path of single elements.
+MANY_ROWS = [(4801, 264), (4737, 136), (5003, 512), (4999, 333), (6001, 131), (9475, 264), (2371, 1024), (3001, 640), (2500, 900),
+             (3001, 264), (4700, 448), (2999, 250)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("shape", MANY_ROWS)
+def test_many_short_rows(ctx, dtype, residual, shape):
+    x0, z0, g0 = inputs(shape, 88)
+    x = bs.Placed(ctx, shape, dtype, values=x0)
+    z = bs.Placed(ctx, shape, dtype, values=z0) if residual else None
+    h = bs.Placed(ctx, shape, dtype) if residual else None
+    gamma = bs.Placed(ctx, (shape[1],), "float32", values=g0)
+    y, s = bs.Placed(ctx, shape, "float8_e4m3"), bs.Placed(ctx, (shape[0], bs.blocks(shape[1])), "float32")
+    bs.rms_norm_quantize(ctx, x, z, h, gamma, EPSILON, y, s)
+    check(x.values, z.values if residual else None, gamma.values, h, y, s, dtype)
+    assert np.array_equal(x.download(), x.values)
+
+
+@pytest.mark.parametrize("offsets", [(2, 0, 0, 0, 0), (0, 4, 0, 0, 0), (0, 0, 8, 0, 0), (0, 0, 0, 4, 0), (0, 0, 0, 0, 3)])
+def test_many_short_rows_in_unaligned_views(ctx, offsets):
+    shape = (4801, 264)
+    x0, z0, g0 = inputs(shape, 89)
+    x, z = bs.Placed(ctx, shape, "bfloat16", offsets[0], values=x0), bs.Placed(ctx, shape, "bfloat16", offsets[1], values=z0)
+    h, gamma = bs.Placed(ctx, shape, "bfloat16", offsets[2]), bs.Placed(ctx, (shape[1],), "float32", offsets[3], values=g0)
+    y, s = bs.Placed(ctx, shape, "float8_e4m3", offsets[4]), bs.Placed(ctx, (shape[0], 3), "float32", 4)
+    bs.rms_norm_quantize(ctx, x, z, h, gamma, EPSILON, y, s)
+    check(x.values, z.values, gamma.values, h, y, s, "bfloat16")
+
+
+def test_nan_and_infinity_among_many_short_rows(ctx):
+    """a row's NaN does not reach its neighbours in the same warp, whichever half of it they are in"""
+    shape = (4801, 264)
+    x0, _, g0 = inputs(shape, 90)
+    bad = np.array([0, 1, 6, 33, 4799, 4800])
+    x0[bad, [0, 263, 130, 255, 8, 256]] = [np.nan, np.nan, np.inf, -np.inf, np.nan, np.inf]
+    x = bs.Placed(ctx, shape, "float16", values=x0)
+    gamma = bs.Placed(ctx, (264,), "float32", values=g0)
+    y, s = bs.Placed(ctx, shape, "float8_e4m3"), bs.Placed(ctx, (4801, 3), "float32")
+    bs.rms_norm_quantize(ctx, x, None, None, gamma, EPSILON, y, s)
+    q, scales = y.download(), s.download()
+    assert np.all(np.any(np.isnan(q[bad]), axis=1))
+    keep = np.setdiff1d(np.arange(4801), bad)
+    _, y64 = o.rms_norm(x.values[keep], None, gamma.values, EPSILON)
+    spread = o.spread_scales(scales[keep], len(keep), 264)
+    assert np.all(np.abs(q[keep] * spread - y64) <= bs.code_error_bound(y64, spread, norm_bound(264) + 2 * bs.U32))
+    assert y.guards_intact() and s.guards_intact()
