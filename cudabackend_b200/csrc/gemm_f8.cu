@@ -8,9 +8,13 @@
  * P_g comes from tcgen05.mma kind::f8f6f4 (products exact, float32 accumulators in TMEM).  The scales are arbitrary float32
  * numbers, which the tensor core cannot apply, so every block of 128 gets an accumulator of its own and a "promotion" in
  * float32 registers, acc += scale * P_g: one read of the accumulator and one fused multiply-add per result and block, on the CUDA
- * cores, beside the MMAs of the next block.  scale = aScale * bScale is formed first and has float32's range; scales from 2^-63 to 2^63 never
- * meet its ends.  Two steps, (P_g * aScale) * bScale with exact powers of two in between, for the blocks that need them would widen it,
- * but looking for such blocks in the promotion costs 3 to 17% (8192^3: 581 us, 597 to 687 us in six forms).  Measured against float64 the result is off by 6e-8 (float32 C, 333 x 2056 x 1616).
+ * cores, beside the MMAs of the next block.  An element is off by at most (min(K, 128) + blocks + 4) * 2^-23 of the sum of its terms'
+ * magnitudes (what the tests allow); the root mean square of the error over that of the result was 6e-8 for float32 C of 333 x 2056 x
+ * 1616.
+ *
+ * scale = aScale * bScale is formed first and has float32's range; scales from 2^-63 to 2^63 never meet its ends.  Two steps, (P_g *
+ * aScale) * bScale with exact powers of two in between, for the blocks that need them would widen it, but looking for such blocks in
+ * the promotion costs 3 to 17% (8192^3: 581 us, 597 to 687 us in six forms).
  *
  * Two kernels: kernel_gemm_f8_split (few rows of A, unaligned rows, few tiles; K split over a cluster) and kernel_gemm_f8_pair (256 x
  * 256 tiles on CTA pairs).  The choice is in launch(), with both sides measured.
@@ -115,8 +119,10 @@ namespace
 	 * that a handful of tokens does not waste 128-row tiles; the result is transposed on the way out.
 	 *
 	 * Bound: the bytes of B in principle; at these sizes the set-up (1000 cycles), the first copy (1200) and the end (1500) of a CTA
-	 * that lives 8000 cycles.  Measured in a graph: 1 x 4096 x 4096 4.8 us (3.5 TB/s), 13 x 8192 x 4096 9.1 us (3.7 TB/s), 1 x 8192 x
-	 * 8192 13.1 us (5.1 TB/s), 128 x 4096 x 4096 9.8 us, 333 x 2056 x 1616 10.1 us.  One tile of 128 rows of B per CTA leaves most SMs without work at the usual sizes, so the blocks of
+	 * that lives 8000 cycles.  Measured in a graph, with more than 330 MB of weights in rotation (from HBM, as a decoding step finds
+	 * them) / with two sets (from L2 where both fit): 1 x 4096 x 4096 6.0 / 4.7 us (2.8 TB/s from HBM), 13 x 8192 x 4096 9.1 / 6.3 us (3.7
+	 * TB/s), 1 x 8192 x 8192 13.2 / 13.2 us (5.1 TB/s).  With two sets: 129 x 2048 x 4096 9.7 us, 333 x 2056 x 1616 10.0 us.
+	 * One tile of 128 rows of B per CTA leaves most SMs without work at the usual sizes, so the blocks of
 	 * K are split over the CTAs of a cluster.  Each CTA finishes a share of the tokens and adds everybody's partial sums for these in
 	 * the order of the ranks: no scratch memory, no atomics, the same bits every time.
 	 *
@@ -1168,9 +1174,10 @@ namespace
 			const cudaError_t launched = launch_chained(kernel_scale_c, grid, dim3(256), 0, ctx.getStream(), p);
 			return launched != cudaSuccess ? convertStatus(launched) : checkForErrors();
 		}
-		/* Few tiles leave most pairs idle, and 256-row tiles waste what few rows of A do not fill.  bfloat16 C, us, pairs / split:
-		 * 256 x 4096 x 4096 (16 tiles) 20.4 / 14.6, 1024^3 (16) 8.5 / 8.6, 333 x 2056 x 1616 (18) 11.2 / 10.1, 512 x 4096 x 4096 (32)
-		 * 20.9 / 21.2, 4096 x 512 x 4096 (32) 21.1 / 27.1, 2048^3 (64) 13.9 / 25.6. */
+		/* Few tiles leave most pairs idle, and 256-row tiles waste what few rows of A do not fill.  bfloat16 C, us in a graph, pairs / split:
+		 * 129 x 2048 x 4096 (8 tiles) 19.2 / 9.7, 256 x 4096 x 4096 (16) 19.6 / 14.0, 1024^3 (16) 8.4 / 8.5, 333 x 2056 x 1616 (18) 11.1 / 10.0,
+		 * 129 and 256 x 8192 x 4096 (32) 20.2 / 22.0 and 20.5 / 22.3, 512 x 4096 x 4096 (32) 20.0 / 22.0, 4096 x 512 x 4096 (32) 20.1 / 22.0,
+		 * 2048^3 (64) 13.2 / 28.2. */
 		const bool tma = p.K % 16 == 0 and (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0;
 		if (tma and p.M > 128 and static_cast<long long>((p.M + 255) / 256) * ((p.N + 255) / 256) >= 32)
 			return launch_pair(ctx, p);

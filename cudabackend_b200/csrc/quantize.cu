@@ -12,10 +12,12 @@
  * NaN reaches its block's scale.  The product x * (448 / a) is at most 448 * (1 + 2^-23), which rounds to 448, so nothing
  * saturates.  All arithmetic is float32; the only other roundings are those of the codes and of the stored sum h.
  *
- * Bound: HBM.  Measured (of 6566 GB/s copied): 4096 x 8192 bfloat16 to 1 x 128 blocks 20.8 us (102 MB, 0.74; a plain copy of that
- * size takes 20 us), 8192 x 8192 to 128 x 128 blocks 34.9 us (201 MB, 0.88), norm of 8192 x 8192 with residual 80 us (470 MB, 0.89),
- * norm of 50176 x 264 float16 14.3 us (40 MB, 0.43: instructions, over 200 per row; a block's work does not shrink with its 8 of 128
- * columns).
+ * Bound: HBM.  Measured in graphs (of 6566 GB/s copied): 4096 x 8192 bfloat16 to 1 x 128 blocks 20.0 us (102 MB, 0.77), 8192 x 8192 to 128
+ * x 128 blocks 33.6 us (201 MB, 0.91), norm of 8192 x 8192 with residual 81 us (470 MB, 0.88), norm of 50176 x 264 float16 13.7 us (40 MB,
+ * 0.44: instructions, over 200 per row; a block's work does not shrink with its 8 of 128 columns).
+ * Not bound by HBM: rows that cannot be moved in 16-byte pieces, whose elements and codes go one by one (8192 x 8191 bfloat16 to 1 x 128
+ * blocks 150 us, 0.20, float32 62 us, 0.82; norm with residual 169 us, 0.42), and norms of more than 8192 columns, whose blocks of 512 or
+ * 1024 threads leave a thread 64 registers for four blocks (4096 x 16384 bfloat16 with residual 126 us, 0.57; float32 160 us, 0.83).
  */
 #include <Avocado/cuda_backend_ext.h>
 
@@ -626,10 +628,11 @@ namespace
 	avStatus_t launch_norm(ContextObject &ctx, const NormArgs &a)
 	{
 		const int blocks = scale_blocks(a.columns);
-		/* Half-warps per row: enough that each holds at most four blocks, or two where that makes 64 to 256 threads of a row (4096 x
-		 * 4096 bfloat16: 27 us with two, 29.5 with four; 8192 x 8192: 110 us with two, 102 with four; 50176 x 264: 26 with two, 17
-		 * with four).  While the rows do not fill the machine, as many as there are blocks, because then the time of one row is the
-		 * time of the call. */
+		/* Half-warps per row: enough that each holds at most four blocks, or two where that makes 64 to 256 threads of a row.  bfloat16 with
+		 * residual, us in a graph with at most two / four: 8192 x 2048 21.7 / 23.8, 4096 x 4096 22.8 / 22.5, 16384 x 1024 22.8 / 22.0, 8192 x 4096
+		 * 41.7 / 39.9, 16384 x 640 19.7 / 16.2: two gains from 9 to 16 blocks only.  Outside that range 4096 x 5120 46.8 / 32.2, 8192 x 8192 101 /
+		 * 80, 50176 x 264 float16 19.4 / 13.6.  While the rows do not fill the machine, as many half-warps as there are blocks, because then
+		 * the time of one row is the time of the call. */
 		const int most_items = (blocks > 4 and blocks <= 32) ? 2 : 4;
 		int halves = 1;
 		const long long room = static_cast<long long>(sm_count(ctx)) * (1024 / kLanes);
