@@ -1051,16 +1051,24 @@ namespace
 		return umma::make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 	}
 
+	/* how many clusters of each size run at once: a cluster stays within a group of SMs and a CTA fills an SM, so SMs are left over in
+	 * each group (148 SMs hold 45 clusters of three, 33 of four, 15 of eight) */
+	struct ClustersAtOnce
+	{
+			int of_size[kMaxSplits + 1];
+	};
 	/* CTAs per tile: the number that ends first, where a CTA's time is its blocks of K (about 350 cycles each) plus that of
-	 * kOverhead blocks for set-up, first copy and reduction, and one CTA runs per SM. */
-	int choose_splits(long long tiles, int blocks, int sms)
+	 * kOverhead blocks for set-up, first copy and reduction. */
+	int choose_splits(long long tiles, int blocks, const ClustersAtOnce &clusters)
 	{
 		constexpr int kOverhead = 6;
 		int best = 1;
 		long long best_cost = 0;
 		for (int s = 1; s <= std::min(kMaxSplits, blocks); s++)
 		{
-			const long long waves = (tiles + sms / s - 1) / (sms / s);
+			if (clusters.of_size[s] < 1)
+				continue;
+			const long long waves = (tiles + clusters.of_size[s] - 1) / clusters.of_size[s];
 			const long long cost = waves * ((blocks + s - 1) / s + kOverhead);
 			if (s == 1 or cost < best_cost)
 			{
@@ -1076,8 +1084,34 @@ namespace
 	{
 		using Cfg = SplitConfig<TOKENS, LOADERS>;
 		auto kernel = kernel_gemm_f8_split<TOKENS, LOADERS>;
+		cudaLaunchConfig_t config = { };
+		config.blockDim = dim3(Cfg::kThreads);
+		config.dynamicSmemBytes = Cfg::kSmemBytes;
+		cudaLaunchAttribute attributes[2];
+		config.attrs = attributes;
+		attributes[0].id = cudaLaunchAttributeClusterDimension;
+		attributes[0].val.clusterDim.y = 1;
+		attributes[0].val.clusterDim.z = 1;
 		static PerDeviceOnce configured;
-		if (configured.run(ctx.device, [&]() -> cudaError_t { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes); }) != cudaSuccess)
+		static ClustersAtOnce clusters[kMaxDevices];
+		const cudaError_t ready = configured.run(ctx.device, [&]() -> cudaError_t
+		{
+			const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+			clusters[ctx.device].of_size[1] = sm_count(ctx);
+			for (int s = 2; status == cudaSuccess and s <= kMaxSplits; s++)
+			{
+				attributes[0].val.clusterDim.x = static_cast<unsigned>(s);
+				config.gridDim = dim3(static_cast<unsigned>(s));
+				config.numAttrs = 1;
+				if (cudaOccupancyMaxActiveClusters(&clusters[ctx.device].of_size[s], kernel, &config) != cudaSuccess)
+				{
+					cudaGetLastError();
+					clusters[ctx.device].of_size[s] = 0; /* such clusters are not used */
+				}
+			}
+			return status;
+		});
+		if (ready != cudaSuccess)
 		{
 			cudaGetLastError();
 			return AVOCADO_STATUS_EXECUTION_FAILED;
@@ -1087,22 +1121,15 @@ namespace
 			return AVOCADO_STATUS_INTERNAL_ERROR;
 		const long long token_tiles = (static_cast<long long>(p.M) + TOKENS - 1) / TOKENS;
 		const long long tiles = token_tiles * scale_blocks(p.N);
-		const int splits = choose_splits(tiles, p.blocks, sm_count(ctx));
+		const int splits = choose_splits(tiles, p.blocks, clusters[ctx.device]);
 		if (tiles * splits > 0x7FFFFFFFll)
 			return AVOCADO_STATUS_NOT_SUPPORTED;
-		cudaLaunchConfig_t config = { };
 		config.gridDim = dim3(static_cast<unsigned>(tiles * splits));
-		config.blockDim = dim3(Cfg::kThreads);
-		config.dynamicSmemBytes = Cfg::kSmemBytes;
 		config.stream = ctx.getStream();
-		cudaLaunchAttribute attributes[2];
-		attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-		attributes[0].val.programmaticStreamSerializationAllowed = chained_launches_enabled() ? 1 : 0;
-		attributes[1].id = cudaLaunchAttributeClusterDimension;
-		attributes[1].val.clusterDim.x = static_cast<unsigned>(splits);
-		attributes[1].val.clusterDim.y = 1;
-		attributes[1].val.clusterDim.z = 1;
-		config.attrs = attributes;
+		attributes[0].val.clusterDim.x = static_cast<unsigned>(splits);
+		cudaLaunchAttribute &chained = attributes[splits > 1 ? 1 : 0];
+		chained.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+		chained.val.programmaticStreamSerializationAllowed = chained_launches_enabled() ? 1 : 0;
 		config.numAttrs = splits > 1 ? 2 : 1;
 		const cudaError_t launched = cudaLaunchKernelEx(&config, kernel, mapA, mapB, p, static_cast<int>(token_tiles), splits, (p.blocks + splits - 1) / splits,
 				ctx.getDeviceStatus());

@@ -389,3 +389,18 @@ def test_zero_scales_and_infinite_ones(ctx, shape):
     assert np.all(np.isnan(got[2, :128])) and np.all(np.isposinf(got[2, 128:]))
     keep = np.arange(m) != 2
     assert np.all(got[keep, :128] == 0.0) and np.array_equal(got[keep, 128:], ref[keep, 128:])
+
+
+@pytest.mark.parametrize("m", [1, 70])
+@pytest.mark.parametrize("tiles", [1, 14, 15, 16, 18, 19, 22, 23, 26, 27, 33, 34, 45, 46, 74, 75, 149])
+def test_tile_counts_around_what_clusters_of_each_size_hold(ctx, m, tiles):
+    """the number of shares of K follows from how many clusters of each size the device runs at once; integers, so any share shows"""
+    n, k = tiles * 128 - 8, 1152
+    p = Problem(ctx, m, n, k, "float32")
+    r = np.random.default_rng(97)
+    p.a.upload(r.integers(-8, 9, (m, k)))
+    p.b.upload(r.integers(-8, 9, (n, k)))
+    p.sa.upload(np.exp2(r.integers(-2, 2, (m, bs.blocks(k)))))
+    p.sb.upload(np.exp2(r.integers(-2, 2, (bs.blocks(n), bs.blocks(k)))))
+    p.run()
+    assert np.array_equal(p.c.download(), p.expected()[0]) and p.c.guards_intact()
