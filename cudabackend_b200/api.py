@@ -6,6 +6,7 @@ write by hand.  There is no fallback of any kind: if the shared library is missi
 is raised.
 """
 import ctypes
+import operator
 import os
 
 import numpy as np
@@ -263,10 +264,15 @@ class Address(int):
         return self
 
     def __add__(self, offset):
-        total = int(self) + offset
-        return Address(total, self.memory) if isinstance(total, int) else total
+        try:
+            return Address(int(self) + operator.index(offset), self.memory)
+        except TypeError:
+            return NotImplemented
 
     __radd__ = __add__
+
+    def __reduce__(self):
+        return int, (int(self),)  # a copy of the number alone
 
 
 class Memory:

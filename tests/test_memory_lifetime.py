@@ -39,6 +39,18 @@ def test_an_address_keeps_its_memory(destroyed):
     assert destroyed == [7]
 
 
+def test_an_address_is_a_number_like_any_other(destroyed):
+    import ctypes
+    import pickle
+    address = api.Memory(64, handle=7).pointer()
+    assert ctypes.c_void_p(address).value == 0x7000 and "%#x" % address == "0x7000" and {address: 1}[0x7000] == 1
+    assert address - 0x6000 == 0x1000 and 16 + address == 0x7010 and address + 0.5 == 28672.5
+    inside = address + np.int64(8)
+    assert inside.memory is address.memory and inside == 0x7008
+    copy = pickle.loads(pickle.dumps(address))
+    assert type(copy) is int and copy == 0x7000
+
+
 def test_destroy_frees_whoever_holds_the_address(destroyed):
     memory = api.Memory(64, handle=7)
     address = memory.pointer()
